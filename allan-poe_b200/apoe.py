@@ -19,6 +19,7 @@ CREATE_FOR_BUILD = 1
 BUILD_SIMT_JOIN, BUILD_KEEP_KNN, BUILD_RANDOM_START, BUILD_SHARED_PAIRS, BUILD_REVERSE_PASS = 1, 2, 4, 8, 16
 BUILD_PRUNE_STEPWISE, BUILD_TRACE, BUILD_DETERMINISTIC, BUILD_WIPE_TABLES = 32, 64, 128, 256
 SEARCH_KEYWORD, SEARCH_KG, SEARCH_RAW_WEIGHTS, SEARCH_UNFUSED_DENSE = 1, 2, 4, 8
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 DIM, ROW, DEGREE, KNN, ENTRY_POINTS = 1024, 40, 32, 64, 32
 
 
@@ -84,6 +85,10 @@ class SearchStats(C.Structure):
                 ("d2h_bytes_hi", C.c_uint32), ("reserved", C.c_uint32 * 3)]
 
 
+class ScaledRows(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("q", C.c_void_p), ("ldq", C.c_uint64), ("scale", C.c_void_p), ("ld_scale", C.c_uint64)]
+
+
 def lib_path() -> str:
     return os.path.join(_HERE, "lib", "libapoe.so")
 
@@ -99,6 +104,14 @@ def lib() -> C.CDLL:
         L.ap_last_error.restype = C.c_char_p
         L.ap_ndcg.restype = C.c_double
         L.ap_index_size.restype = C.c_uint32
+        u32, u64, vp, f32, sz = C.c_uint32, C.c_uint64, C.c_void_p, C.c_float, C.c_size_t
+        L.ap_dense_check_status.argtypes = [C.c_int, vp]
+        L.ap_quantize_rows_device.argtypes = [C.c_int, u32, u32, u32, vp, u64, vp, u64, vp, u64, vp]
+        L.ap_scaled_scores_device.argtypes = [C.c_int, u32, C.POINTER(ScaledRows), C.POINTER(ScaledRows), f32, u32, vp, u64, vp]
+        L.ap_softmax_loss_workspace.argtypes = [C.c_int, u32, u32, u32, C.c_int, C.POINTER(sz)]
+        L.ap_softmax_loss_forward_device.argtypes = [C.c_int, u32, u32, u32, u32, vp, u64, vp, u64, vp, f32, vp, vp, vp, sz, vp]
+        L.ap_softmax_loss_backward_device.argtypes = [C.c_int, u32, u32, u32, u32, vp, u64, vp, u64, vp, f32, vp, vp, vp, vp, u64, vp, u64,
+                                                      vp, sz, vp]
         _LIB = L
     return _LIB
 
@@ -434,6 +447,150 @@ class Index:
         _check(lib().ap_fused_distances(self._h, C.byref(q), C.byref(o), C.c_size_t(pq.size), _ptr(pq), _ptr(pd),
                                         _ptr(out)))
         return out
+
+
+# ---- dense operators (CUDA tensors in and out, on the current stream of their device) ---------------------------------
+_TYPES = {}
+
+
+def _type_of(dtype) -> int:
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
+    try:
+        return _TYPES[dtype]
+    except KeyError:
+        raise ApoeError(1, f"{dtype}: float32, float16 and bfloat16 are supported") from None
+
+
+def _matrix(name, t, device=None, dtypes=None):
+    """(device index, rows, columns, row stride) of a CUDA matrix whose rows are contiguous."""
+    if t.dim() != 2 or not t.is_cuda:
+        raise ApoeError(1, f"{name}: a CUDA matrix is needed, got {tuple(t.shape)} on {t.device}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ApoeError(1, f"{name}: the values of a row must be contiguous")
+    if device is not None and t.device.index != device:
+        raise ApoeError(1, f"{name}: is on {t.device}, the other tensors on cuda:{device}")
+    if dtypes is not None and t.dtype not in dtypes:
+        raise ApoeError(1, f"{name}: {t.dtype} where {' or '.join(map(str, dtypes))} is needed")
+    rows, cols = t.shape
+    ld = t.stride(0) if rows > 1 else max(t.stride(0), cols)
+    if ld < cols:
+        raise ApoeError(1, f"{name}: rows overlap (stride {ld}, {cols} values)")
+    return t.device.index, rows, cols, ld
+
+
+def _vector(name, t, n, device, dtypes):
+    if t.dim() != 1 or t.shape[0] != n or not t.is_cuda or t.device.index != device or not t.is_contiguous() or t.dtype not in dtypes:
+        raise ApoeError(1, f"{name}: a contiguous vector of {n} {' or '.join(map(str, dtypes))} on cuda:{device} is needed, "
+                           f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _stream(device, stream):
+    if stream is not None:
+        return stream
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def quantize_rows(x, stream=None):
+    """Rows in 8 bits: (q float8_e4m3fn [rows, dim], scale uint8 [rows, ceil(dim / 128)]).  The value of q[r, c] is
+    q * 2^(scale[r, c // 128] - 127).  x: float32, float16 or bfloat16 matrix.  The rows of q start on 16-byte boundaries."""
+    import torch
+    kind = _type_of(x.dtype)
+    device, rows, dim, ld = _matrix("x", x)
+    if dim == 0:
+        raise ApoeError(1, "quantize: rows of 0 values")
+    ldq, blocks = (dim + 15) // 16 * 16, (dim + 127) // 128
+    q = torch.empty(rows, ldq, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(rows, blocks, dtype=torch.uint8, device=x.device)
+    _check(lib().ap_quantize_rows_device(device, rows, dim, kind, x.data_ptr(), ld, q.data_ptr(), ldq, scale.data_ptr(), blocks,
+                                         _stream(device, stream)))
+    return (q if ldq == dim else q[:, :dim]), scale
+
+
+def scaled_scores(a, a_scale, b, b_scale, out_dtype=None, alpha: float = 1.0, out=None, stream=None):
+    """Scores of 8-bit rows (as `quantize_rows` returns them): [rows of a, rows of b] in out_dtype (float32 by default,
+    float16, bfloat16), summed in fp32.  Rows of a and b must start on 16-byte boundaries."""
+    import torch
+    f8, u8 = (torch.float8_e4m3fn,), (torch.uint8,)
+    device, m, dim, lda = _matrix("a", a, None, f8)
+    _, n, dim_b, ldb = _matrix("b", b, device, f8)
+    if dim != dim_b:
+        raise ApoeError(1, f"scores: rows of {dim} and of {dim_b} values")
+    blocks = (dim + 127) // 128
+    _, ma, ca, lsa = _matrix("a_scale", a_scale, device, u8)
+    _, nb, cb, lsb = _matrix("b_scale", b_scale, device, u8)
+    if (ma, ca, nb, cb) != (m, blocks, n, blocks):
+        raise ApoeError(1, f"scores: scales {ma} x {ca} and {nb} x {cb}, needed {m} x {blocks} and {n} x {blocks}")
+    if out is None:
+        out = torch.empty(m, n, dtype=out_dtype or torch.float32, device=a.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ApoeError(1, f"scores: out is {out.dtype}, out_dtype {out_dtype}")
+    kind = _type_of(out.dtype)
+    _, om, on, ldo = _matrix("out", out, device)
+    if (om, on) != (m, n):
+        raise ApoeError(1, f"scores: out is {om} x {on}, needed {m} x {n}")
+    ra = ScaledRows(m, a.data_ptr(), lda, a_scale.data_ptr(), lsa)
+    rb = ScaledRows(n, b.data_ptr(), ldb, b_scale.data_ptr(), lsb)
+    _check(lib().ap_scaled_scores_device(device, dim, ra, rb, alpha, kind, out.data_ptr(), ldo, _stream(device, stream)))
+    return out
+
+
+def _loss_args(queries, docs, target):
+    import torch
+    half = (torch.float16, torch.bfloat16)
+    device, rows, dim, ldq = _matrix("queries", queries, None, half)
+    _, n, dim_d, ldd = _matrix("docs", docs, device, (queries.dtype,))
+    if dim != dim_d:
+        raise ApoeError(1, f"softmax loss: queries of {dim} values, documents of {dim_d}")
+    _vector("target", target, rows, device, (torch.int32, torch.uint32))
+    return device, rows, n, dim, _type_of(queries.dtype), ldq, ldd
+
+
+def _workspace(device, rows, n, dim, backward):
+    import torch
+    size = C.c_size_t(0)
+    _check(lib().ap_softmax_loss_workspace(device, rows, n, dim, backward, size))
+    return torch.empty(size.value, dtype=torch.uint8, device=torch.device("cuda", device)), size.value
+
+
+def softmax_loss_forward(queries, docs, target, scale: float = 1.0, stream=None):
+    """Softmax loss of queries over all documents without holding the matrix of scores: (loss, lse), float32 [rows].
+    queries [rows, dim] and docs [n, dim]: float16 or bfloat16; target: int32 document ids, -1 = the row takes no part."""
+    import torch
+    device, rows, n, dim, kind, ldq, ldd = _loss_args(queries, docs, target)
+    out = torch.empty(2, rows, dtype=torch.float32, device=queries.device)
+    loss, lse = out[0], out[1]
+    ws, size = _workspace(device, rows, n, dim, 0)
+    _check(lib().ap_softmax_loss_forward_device(device, rows, n, dim, kind, queries.data_ptr(), ldq, docs.data_ptr(), ldd, target.data_ptr(),
+                                                scale, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size, _stream(device, stream)))
+    return loss, lse
+
+
+def softmax_loss_backward(queries, docs, target, loss, lse, grad_loss, scale: float = 1.0, stream=None):
+    """Gradients of `softmax_loss_forward`: (grad_queries, grad_docs) in the vectors' type.  loss, lse: as the forward call
+    returned them; grad_loss: float32 [rows], the gradient of each row's loss (1 / rows for a mean)."""
+    import torch
+    device, rows, n, dim, kind, ldq, ldd = _loss_args(queries, docs, target)
+    f32 = (torch.float32,)
+    _vector("loss", loss, rows, device, f32)
+    _vector("lse", lse, rows, device, f32)
+    _vector("grad_loss", grad_loss, rows, device, f32)
+    pad = (dim + 7) // 8 * 8
+    gq = torch.empty(rows, pad, dtype=queries.dtype, device=queries.device)
+    gd = torch.empty(n, pad, dtype=queries.dtype, device=queries.device)
+    ws, size = _workspace(device, rows, n, dim, 1)
+    _check(lib().ap_softmax_loss_backward_device(device, rows, n, dim, kind, queries.data_ptr(), ldq, docs.data_ptr(), ldd, target.data_ptr(),
+                                                 scale, loss.data_ptr(), lse.data_ptr(), grad_loss.data_ptr(), gq.data_ptr(), pad,
+                                                 gd.data_ptr(), pad, ws.data_ptr(), size, _stream(device, stream)))
+    return (gq, gd) if pad == dim else (gq[:, :dim], gd[:, :dim])
+
+
+def dense_check_status(device: int = 0, stream=None) -> None:
+    """Waits for the stream (the device's current one by default) and raises ApoeError(6) when a bounded wait of an earlier
+    dense operator ran out."""
+    _check(lib().ap_dense_check_status(device, _stream(device, stream)))
 
 
 def build_index(dense_path, sparse_path, bm25_path, out_path, device=0, iterations=0, seed=0, flags=0) -> BuildStats:

@@ -11,7 +11,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC"]
-CU_SOURCES = ["apoe_index.cu", "apoe_search.cu", "apoe_build.cu", "apoe_join_tc.cu", "apoe_prep.cu", "apoe_exact.cu", "apoe_files.cpp"]
+CU_SOURCES = ["apoe_index.cu", "apoe_search.cu", "apoe_build.cu", "apoe_join_tc.cu", "apoe_prep.cu", "apoe_exact.cu", "apoe_dense.cu",
+              "apoe_files.cpp"]
 
 
 def _nvcc() -> str:
@@ -40,7 +41,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(LIBDIR, exist_ok=True)
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    headers = [os.path.join(CSRC, "apoe_common.cuh"), os.path.join(HERE, "..", "include", "allan_poe.h")]
+    headers = [os.path.join(CSRC, "apoe_common.cuh"), os.path.join(CSRC, "apoe_tile.cuh"), os.path.join(HERE, "..", "include", "allan_poe.h")]
     objs, procs = [], []
     for src in CU_SOURCES:
         sp = os.path.join(CSRC, src)

@@ -1,0 +1,787 @@
+// Operators over dense query and document vectors: 8-bit rows with a power-of-two scale for each block of 128 values, the
+// scores of such rows against each other, and the softmax loss of queries over all documents with its gradients.
+//
+//   quantize    q = e4m3(x 2^-e), e the smallest exponent (>= -126) with max |x| of the block <= 448 * 2^e
+//   scores      S = alpha * sum over blocks of 2^(ea + eb) <qa, qb>
+//   loss        l[t][v] = scale <x_t, w_v>;  lse_t = log sum_v exp l[t][v];  loss_t = lse_t - l[t][target_t]
+//   gradients   G[t][v] = grad_t (exp(l[t][v] - lse_t) - [v = target_t]);  dX = scale G W;  dW = scale G^T X
+//
+// The products run on the tile engine (apoe_tile.cuh).  Neither the scores' scaled operands nor the logits of the loss are
+// ever held whole: the loss keeps a running maximum and sum per row and column tile, the gradients recompute the logits of
+// one piece of the documents at a time.
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+
+#include "apoe_tile.cuh"
+
+namespace apoe {
+
+using tile::Grid;
+using tile::Scales;
+
+constexpr uint32_t kNoTarget = 0xFFFFFFFFu;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr uint32_t kAll = 0xFFFFFFFFu;
+
+__device__ uint32_t dense_error_word;   // raised by a kernel whose bounded wait ran out; read by ap_dense_check_status
+
+struct DeviceScope {   // calls leave the caller's current device as it was
+    int prev = -1;
+    ~DeviceScope() { if (prev >= 0) cudaSetDevice(prev); }
+    int enter(int device) {
+        AP_CUDA(cudaGetDevice(&prev));
+        if (prev == device) { prev = -1; return AP_OK; }
+        const cudaError_t e = cudaSetDevice(device);
+        if (e != cudaSuccess) { prev = -1; return fail(AP_ERR_CUDA, "cudaSetDevice(%d) failed: %s", device, cudaGetErrorString(e)); }
+        return AP_OK;
+    }
+};
+
+template <class T> struct Half16;
+template <> struct Half16<__half> {
+    static constexpr int kind = tile::kF16;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_half2(lo, hi); }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
+    static __device__ __forceinline__ __half cast(float v) { return __float2half_rn(v); }
+};
+template <> struct Half16<__nv_bfloat16> {
+    static constexpr int kind = tile::kBf16;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&p);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&v)); }
+    static __device__ __forceinline__ __nv_bfloat16 cast(float v) { return __float2bfloat16_rn(v); }
+};
+
+// ---------------------------------------------------------------------------------------------------------------------
+// 8-bit rows
+// ---------------------------------------------------------------------------------------------------------------------
+// Exponent of a block from its largest magnitude a = 1.f * 2^E: the smallest e with a <= 448 * 2^e = 1.75 * 2^(e + 8), kept
+// at or above -126 so that 2^-e is a normal float (blocks below 448 * 2^-126 then use fewer of the 8 bits).  Exact: read
+// from the bits.  An infinity counts as 2^128: its quantised value times its scale overflows back to infinity.
+__device__ __forceinline__ int block_exponent(float a) {
+    const uint32_t b = __float_as_uint(a);
+    return max((int)(b >> 23) - 127 - ((b & 0x7FFFFFu) <= 0x600000u ? 8 : 7), -126);
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {   // nearest even; beyond 448: 448; NaN stays NaN
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <class T> __device__ __forceinline__ float load_as_float(const T *p);
+template <> __device__ __forceinline__ float load_as_float<float>(const float *p) { return *p; }
+template <> __device__ __forceinline__ float load_as_float<__half>(const __half *p) { return __half2float(*p); }
+template <> __device__ __forceinline__ float load_as_float<__nv_bfloat16>(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+
+struct QuantArgs {
+    const void *src;
+    uint8_t *q, *scale;
+    size_t lds, ldq, ldsc;     // row strides: elements of src, bytes of q and scale
+    uint64_t items;            // rows x blocks
+    uint32_t dim, blocks;
+    uint32_t vec;              // src and q rows allow 16-byte (f32) / 8-byte (f16, bf16) accesses
+};
+
+// One warp per block of 128 values, kQuantUnroll neighbouring blocks in flight: memory-bound, one pass.  Each lane holds four
+// consecutive values of a block (16 bytes of f32, 8 bytes of f16 / bf16), five shuffles give the block's maximum.
+constexpr int kQuantUnroll = 4;
+template <class T>
+__global__ void __launch_bounds__(256) quantize_kernel(const QuantArgs a) {
+    const int lane = threadIdx.x & 31;
+    const uint64_t w0 = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+    for (uint64_t first = w0 * kQuantUnroll; first < a.items; first += (uint64_t)gridDim.x * (blockDim.x >> 5) * kQuantUnroll) {
+        float v[kQuantUnroll][4];
+        uint64_t row[kQuantUnroll];
+        uint32_t blk[kQuantUnroll];
+#pragma unroll
+        for (int u = 0; u < kQuantUnroll; ++u) {
+            const uint64_t it = first + u;
+            row[u] = it / a.blocks;
+            blk[u] = (uint32_t)(it - row[u] * a.blocks);
+            const uint32_t c = blk[u] * 128 + lane * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[u][i] = 0.0f;
+            if (it < a.items) {
+                const T *p = static_cast<const T *>(a.src) + row[u] * a.lds + c;
+                if (a.vec && c + 4 <= a.dim) {
+                    if constexpr (sizeof(T) == 4) {
+                        const float4 f = __ldcs(reinterpret_cast<const float4 *>(p));
+                        v[u][0] = f.x; v[u][1] = f.y; v[u][2] = f.z; v[u][3] = f.w;
+                    } else {
+                        const uint2 h = __ldcs(reinterpret_cast<const uint2 *>(p));
+                        const float2 lo = Half16<T>::unpack(h.x), hi = Half16<T>::unpack(h.y);
+                        v[u][0] = lo.x; v[u][1] = lo.y; v[u][2] = hi.x; v[u][3] = hi.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) if (c + i < a.dim) v[u][i] = load_as_float(p + i);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kQuantUnroll; ++u) {
+            float m = 0.0f;                                  // a NaN is never taken: fmaxf returns the other one
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(v[u][i]));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+            const int e = block_exponent(m);
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+            if (first + u >= a.items) continue;
+            const uint32_t c = blk[u] * 128 + lane * 4;
+            const uint32_t p = e4m3x2(v[u][0] * down, v[u][1] * down) | (e4m3x2(v[u][2] * down, v[u][3] * down) << 16);
+            uint8_t *o = a.q + row[u] * a.ldq + c;
+            if (a.vec && c + 4 <= a.dim) *reinterpret_cast<uint32_t *>(o) = p;
+            else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if (c + i < a.dim) o[i] = (uint8_t)(p >> (8 * i));
+            }
+            if (lane == 0) a.scale[row[u] * a.ldsc + blk[u]] = (uint8_t)(e + 127);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// epilogues of the tile engine
+// ---------------------------------------------------------------------------------------------------------------------
+// Stores a tile: 32 columns at a time through the warp's 4 KB of shared memory (16-byte units exchanged by row so neither
+// side has bank conflicts), then whole 128-byte (f32) or 64-byte (f16, bf16) pieces of rows.
+template <class T>
+struct StoreEpi {
+    struct Args {
+        T *out;
+        size_t ld, split_stride;     // elements; result of split s starts at out + s * split_stride
+        uint32_t m, n;
+        float alpha;
+        const float *alpha_dev;      // another factor, read on the device (may be null)
+        uint32_t add;                // f32 only: add to what is there
+        uint32_t vec;                // rows of `out` start on 16-byte boundaries
+    };
+    const Args &a;
+    uint8_t *st;
+    int lane;
+    float alpha;
+    uint32_t row0 = 0;
+    T *base = nullptr;
+    __device__ __forceinline__ StoreEpi(const Args &args, uint8_t *staging, int lane_) : a(args), st(staging), lane(lane_) {
+        alpha = a.alpha_dev ? a.alpha * __ldg(a.alpha_dev) : a.alpha;
+    }
+    __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t split, uint32_t) { row0 = r0; base = a.out + split * a.split_stride; }
+    __device__ __forceinline__ void end() {}
+    __device__ __forceinline__ void chunk(uint32_t (&r)[32], uint32_t col) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
+        put(r, col);
+    }
+    __device__ __forceinline__ void put(const uint32_t (&r)[32], uint32_t col) {
+        if (row0 >= a.m || col >= a.n) return;          // uniform over the warp
+        const uint32_t rows = min(32u, a.m - row0), cols = min(32u, a.n - col);
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<uint4 *>(st + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t p[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = Half16<T>::pack(__uint_as_float(r[8 * j + 2 * i]), __uint_as_float(r[8 * j + 2 * i + 1]));
+                *reinterpret_cast<uint4 *>(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
+            }
+        }
+        __syncwarp();
+        constexpr int UNITS = (int)sizeof(T) * 2;       // 16-byte units of a row's 32 columns
+        constexpr int RPI = 32 / UNITS;                 // rows per pass
+        if (a.vec && cols == 32) {
+#pragma unroll
+            for (int i = 0; i < 32 / RPI; ++i) {
+                const int row = i * RPI + lane / UNITS, j = lane % UNITS;
+                const int sw = sizeof(T) == 4 ? (j ^ (row & 7)) : (j ^ ((row >> 1) & 3));
+                uint4 v = *reinterpret_cast<const uint4 *>(st + row * (UNITS * 16) + (sw << 4));
+                if ((uint32_t)row < rows) {
+                    uint4 *o = reinterpret_cast<uint4 *>(base + (size_t)(row0 + row) * a.ld + col) + j;
+                    if constexpr (sizeof(T) == 4) {
+                        if (a.add) {
+                            const float4 w = *reinterpret_cast<const float4 *>(o);
+                            v.x = __float_as_uint(__uint_as_float(v.x) + w.x); v.y = __float_as_uint(__uint_as_float(v.y) + w.y);
+                            v.z = __float_as_uint(__uint_as_float(v.z) + w.z); v.w = __float_as_uint(__uint_as_float(v.w) + w.w);
+                        }
+                    }
+                    *o = v;
+                }
+            }
+        } else if ((uint32_t)lane < cols) {
+            for (uint32_t row = 0; row < rows; ++row) {
+                constexpr int PER = 16 / (int)sizeof(T);
+                const int j = lane / PER, sw = sizeof(T) == 4 ? (j ^ ((int)row & 7)) : (j ^ (((int)row >> 1) & 3));
+                T v = *reinterpret_cast<const T *>(st + row * (UNITS * 16) + (sw << 4) + (lane % PER) * sizeof(T));
+                T *o = base + (size_t)(row0 + row) * a.ld + col + lane;
+                if constexpr (sizeof(T) == 4) { if (a.add) v += *o; }
+                *o = v;
+            }
+        }
+        __syncwarp();
+    }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {   // 2^x, 2 ulp; results below 2^-126 become 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Running maximum and sum of 2^(l log2 e) of a row over the columns of a tile, the target's column left out: the target's
+// own logit is computed on its own, in fp32 over all of K, because the loss is a difference against it.
+struct LseEpi {
+    struct Args {
+        float2 *part;            // [rows][parts]: maximum and sum, in base 2
+        const uint32_t *target;
+        uint32_t parts, m, n, col0;   // col0: document of this piece's first column
+        float c;                 // scale * log2 e
+    };
+    const Args &a;
+    int lane;
+    uint32_t row = 0, part = 0, tgt = 0;
+    float top = 0.f, sum = 0.f;
+    __device__ __forceinline__ LseEpi(const Args &args, uint8_t *, int lane_) : a(args), lane(lane_) {}
+    __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t, uint32_t p) {
+        row = r0 + lane; part = p;
+        tgt = row < a.m ? __ldg(a.target + row) - a.col0 : kNoTarget;   // columns are below 2^31: no match for a target of another piece
+        top = -1.0e30f; sum = 0.f;
+    }
+    __device__ __forceinline__ void chunk(uint32_t (&r)[32], uint32_t col) {
+        float v[32], m = top;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * a.c;
+        const uint32_t at = tgt - col, cols = a.n > col ? a.n - col : 0u;
+        if (__any_sync(kAll, at < 32u) || cols < 32u) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) if (at == (uint32_t)j || (uint32_t)j >= cols) v[j] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) m = fmaxf(m, v[j]);
+        float s0 = sum * exp2_fast(top - m), s1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) { s0 += exp2_fast(v[j] - m); s1 += exp2_fast(v[j + 1] - m); }
+        top = m; sum = s0 + s1;
+    }
+    __device__ __forceinline__ void end() { if (row < a.m) a.part[(size_t)row * a.parts + part] = make_float2(top, sum); }
+};
+
+// One piece of G, times a power of two that brings the largest |grad| to 2^14 (f16 keeps small probabilities normal); a
+// rounding to 16 bits per element, the operands of the two products that follow.
+template <class T>
+struct GradEpi {
+    struct Args {
+        typename StoreEpi<T>::Args out;
+        const uint32_t *target;
+        const float *loss, *lse, *grad;
+        const float *factor;     // the power of two
+        uint32_t col0, docs;
+        float c;
+    };
+    const Args &a;
+    StoreEpi<T> store;
+    uint32_t tgt = 0;
+    float lse2 = 0.f, g = 0.f, at_target = 0.f;
+    __device__ __forceinline__ GradEpi(const Args &args, uint8_t *staging, int lane) : a(args), store(args.out, staging, lane) {}
+    __device__ __forceinline__ void begin(uint32_t r0, uint32_t n0, uint32_t s, uint32_t p) {
+        store.begin(r0, n0, s, p);
+        const uint32_t row = r0 + store.lane;
+        const uint32_t t = row < a.out.m ? __ldg(a.target + row) : kNoTarget;
+        tgt = t - a.col0;
+        g = 0.f; lse2 = 0.f; at_target = 0.f;
+        if (t < a.docs) {
+            g = __ldg(a.grad + row) * __ldg(a.factor);
+            lse2 = __ldg(a.lse + row) * kLog2e;
+            at_target = g * expm1f(-__ldg(a.loss + row));   // -(1 - p) of the target, exact where p is near 1
+        } else tgt = kNoTarget;
+    }
+    __device__ __forceinline__ void end() {}
+    __device__ __forceinline__ void chunk(uint32_t (&r)[32], uint32_t col) {
+        const bool live = g != 0.f;      // rows without a target may hold anything, NaN included: their G is zero
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = live ? __float_as_uint(g * exp2_fast(fmaf(__uint_as_float(r[j]), a.c, -lse2))) : 0u;
+        const uint32_t at = tgt - col;
+        if (__any_sync(kAll, at < 32u)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) if (at == (uint32_t)j) r[j] = __float_as_uint(at_target);
+        }
+        store.put(r, col);
+    }
+};
+
+// ---------------------------------------------------------------------------------------------------------------------
+// loss: joining the tiles, preparing and finishing the gradients
+// ---------------------------------------------------------------------------------------------------------------------
+struct JoinArgs {
+    const float2 *part;
+    float2 *carry;               // [rows] running maximum and sum over the pieces before this one
+    const void *x, *w;
+    size_t ldx, ldw;
+    const uint32_t *target;
+    float *loss, *lse;
+    uint32_t rows, docs, dim, parts, first, last;
+    float scale;
+};
+// One warp per row.  With z = log(sum of the others) - (target's logit): loss = log(1 + e^z), which keeps its digits where the
+// row is nearly certain (z << 0) and where it is hopeless; lse = target's logit + loss.
+template <class T>
+__global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs a) {
+    const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= a.rows) return;
+    float top = -1.0e30f, sum = 0.f;
+    const float2 *p = a.part + (size_t)row * a.parts;
+    for (uint32_t i = lane; i < a.parts; i += 32) {
+        const float2 e = __ldg(p + i);
+        const float m = fmaxf(top, e.x);
+        sum = sum * exp2f(top - m) + e.y * exp2f(e.x - m);
+        top = m;
+    }
+    if (lane == 0 && !a.first) {
+        const float2 e = a.carry[row];
+        const float m = fmaxf(top, e.x);
+        sum = sum * exp2f(top - m) + e.y * exp2f(e.x - m);
+        top = m;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float t2 = __shfl_xor_sync(kAll, top, o), s2 = __shfl_xor_sync(kAll, sum, o);
+        const float m = fmaxf(top, t2);
+        sum = sum * exp2f(top - m) + s2 * exp2f(t2 - m);
+        top = m;
+    }
+    if (!a.last) { if (lane == 0) a.carry[row] = make_float2(top, sum); return; }
+    const uint32_t t = a.target[row];
+    float loss = 0.f, lse = 0.f;
+    if (t < a.docs) {
+        const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx, *w = static_cast<const T *>(a.w) + (size_t)t * a.ldw;
+        float d0 = 0.f, d1 = 0.f;
+        uint32_t i = lane * 8;
+        for (; i + 8 <= a.dim; i += 256) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(x + i)), v = __ldg(reinterpret_cast<const uint4 *>(w + i));
+            const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 fu = Half16<T>::unpack(us[k]), fv = Half16<T>::unpack(vs[k]);
+                d0 = fmaf(fu.x, fv.x, d0); d1 = fmaf(fu.y, fv.y, d1);
+            }
+        }
+        for (; i < a.dim; ++i) { d0 = fmaf(load_as_float(x + i), load_as_float(w + i), d0); if ((i & 7) == 7) break; }
+        float dot = d0 + d1;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(kAll, dot, o);
+        const float at = a.scale * dot;
+        const float z = (log2f(sum) + top) * kLn2 - at;           // sum = 0 (one document): minus infinity, loss 0
+        loss = z > 0.f ? z + log1pf(expf(-z)) : log1pf(expf(z));  // a NaN stays one
+        lse = at + loss;
+    } else if (t != kNoTarget) loss = lse = __int_as_float(0x7FFFFFFF);
+    if (lane == 0) { a.loss[row] = loss; a.lse[row] = lse; }
+}
+
+struct PrepArgs {
+    const void *x;
+    void *xc;
+    size_t ldx, ldxc;
+    const uint32_t *target;
+    const float *grad;
+    float *factor;               // [0] the power of two, [1] scale / that
+    uint32_t rows, docs, dim;
+    float scale;
+};
+// A copy of the query rows with those that have no target set to zero (0 times whatever a padding row holds would not be 0
+// inside a product); block 0 also finds the factor of G from the largest |grad| of the rows that count.
+template <class T>
+__global__ void __launch_bounds__(256) grad_prep_kernel(const PrepArgs a) {
+    if (blockIdx.x == 0) {
+        __shared__ float s[8];
+        float m = 0.f;
+        for (uint32_t i = threadIdx.x; i < a.rows; i += 256) if (a.target[i] < a.docs) m = fmaxf(m, fabsf(a.grad[i]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = m;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int i = 1; i < 8; ++i) m = fmaxf(m, s[i]);
+            int e = 0;
+            if (m > 0.f && m < INFINITY) frexpf(m, &e);            // m <= 2^e
+            const int k = min(max(14 - e, -100), 100);
+            a.factor[0] = ldexpf(1.f, k);
+            a.factor[1] = ldexpf(a.scale, -k);
+        }
+        return;
+    }
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t row = (blockIdx.x - 1) * 8 + (threadIdx.x >> 5); row < a.rows; row += (gridDim.x - 1) * 8) {
+        const bool live = a.target[row] < a.docs;
+        const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx;
+        T *o = static_cast<T *>(a.xc) + (size_t)row * a.ldxc;
+        for (uint32_t i = lane * 8; i < a.dim; i += 256) {
+            if (i + 8 <= a.dim) *reinterpret_cast<uint4 *>(o + i) = live ? __ldg(reinterpret_cast<const uint4 *>(x + i)) : make_uint4(0u, 0u, 0u, 0u);
+            else for (uint32_t k = i; k < a.dim; ++k) o[k] = live ? x[k] : Half16<T>::cast(0.f);
+        }
+    }
+}
+
+struct FinishArgs {
+    const float *part;           // [splits][rows][ldp]
+    const float *factor;
+    void *dx;
+    size_t ldp, ldd;
+    uint32_t rows, dim, splits;
+};
+// dX from the partial sums of the splits (added in a fixed order), rounded once
+template <class T>
+__global__ void __launch_bounds__(256) grad_finish_kernel(const FinishArgs a) {
+    const float f = a.factor[1];
+    const uint32_t quads = (a.dim + 3) / 4;
+    const uint64_t total = (uint64_t)a.rows * quads;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t row = (uint32_t)(i / quads), c = (uint32_t)(i - (uint64_t)row * quads) * 4;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t k = 0; k < a.splits; ++k) {
+            const float4 v = __ldcs(reinterpret_cast<const float4 *>(a.part + ((size_t)k * a.rows + row) * a.ldp + c));
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        T *o = static_cast<T *>(a.dx) + (size_t)row * a.ldd + c;
+        if (c + 4 <= a.dim)
+            *reinterpret_cast<uint2 *>(o) = make_uint2(Half16<T>::pack(s.x * f, s.y * f), Half16<T>::pack(s.z * f, s.w * f));
+        else {
+            const float v[4] = {s.x * f, s.y * f, s.z * f, s.w * f};
+            for (uint32_t k = 0; c + k < a.dim; ++k) o[k] = Half16<T>::cast(v[k]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------------
+// rows x cols values, rows `ld` values apart; box = one 128-byte span of columns x box_rows rows, 128-byte swizzle.  Reads
+// beyond the extents give zeros.
+static int make_map_2d(CUtensorMap *map, int kind, const void *base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
+    EncodeTiledFn fn;
+    AP_TRY(encode_fn(&fn));
+    const uint32_t size = kind == tile::kE4m3 ? 1 : 2;
+    const CUtensorMapDataType t = kind == tile::kE4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                : kind == tile::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {ld * size};
+    const cuuint32_t box[2] = {128 / size, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, t, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(AP_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+    return AP_OK;
+}
+struct Operand {   // a stored matrix: rows x cols, row stride in values
+    const void *base;
+    uint64_t rows, cols, ld;
+};
+static uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+// C[m][n] = sum over k of A B^T on one shape.  K-major operands are stored rows x K, MN-major ones K x rows.
+template <class S, class Epi>
+static int tile_launch(const Operand &a, const Operand &b, uint32_t m, uint32_t n, uint32_t k, uint32_t splits, const Scales &sc,
+                       const typename Epi::Args &epi, int sms, uint32_t *err, cudaStream_t st) {
+    CUtensorMap ma, mb;
+    AP_TRY(make_map_2d(&ma, S::KIND, a.base, a.rows, a.cols, a.ld, S::AMN ? 64 : 128));
+    AP_TRY(make_map_2d(&mb, S::KIND, b.base, b.rows, b.cols, b.ld, S::BMN ? 64 : S::BR));
+    Grid g;
+    g.tiles_m = ceil_div(m, S::M);
+    g.tiles_n = ceil_div(n, S::N);
+    g.splits = splits;
+    g.kblocks = ceil_div(k, S::K);
+    g.total = g.tiles_m * g.tiles_n * splits;
+    // row tiles that walk the columns together: all of them while their operand stays in L2 (32 MB of it), else 8
+    const uint64_t row_bytes = (uint64_t)S::M * k * (S::SCALED ? 1 : 2);
+    g.group_m = std::min<uint32_t>(g.tiles_m, (uint32_t)std::max<uint64_t>(8, (32ull << 20) / row_bytes));
+    AP_CUDA(cudaFuncSetAttribute(tile::tile_kernel<S, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(std::min<uint32_t>(g.total, (uint32_t)sms / S::CG) * S::CG);
+    cfg.blockDim = dim3(tile::kThreads);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = S::CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    AP_CUDA(cudaLaunchKernelEx(&cfg, tile::tile_kernel<S, Epi>, ma, mb, g, sc, epi, err));
+    return AP_OK;
+}
+
+static int device_facts(int device, int *sms, uint32_t **err) {
+    AP_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+    void *p = nullptr;
+    AP_CUDA(cudaGetSymbolAddress(&p, dense_error_word));
+    *err = static_cast<uint32_t *>(p);
+    return AP_OK;
+}
+static bool aligned(const void *p, uint64_t stride_bytes, uint64_t to) { return (uintptr_t)p % to == 0 && stride_bytes % to == 0; }
+static int elem_size(uint32_t type) { return type == AP_TYPE_F32 ? 4 : (type == AP_TYPE_F16 || type == AP_TYPE_BF16) ? 2 : 0; }
+
+// ---- loss: how the work is cut ------------------------------------------------------------------------------------------
+constexpr uint32_t kTileN = 256;
+static size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
+
+struct ForwardPlan { uint32_t piece, parts; size_t part_bytes, bytes; };
+// The tiles' maxima and sums (8 bytes per row and 128 columns) of at most 64 MB of documents at a time
+static ForwardPlan forward_plan(uint32_t rows, uint32_t docs) {
+    ForwardPlan p;
+    const uint64_t fit = (64ull << 20) / ((uint64_t)rows * 16) * kTileN;
+    p.piece = (uint32_t)std::min<uint64_t>((uint64_t)ceil_div(docs, kTileN) * kTileN, std::max<uint64_t>(fit, 32 * kTileN));
+    p.parts = 2 * ceil_div(std::min(p.piece, docs), kTileN);
+    p.part_bytes = round256((size_t)rows * p.parts * 8);
+    p.bytes = p.part_bytes + round256((size_t)rows * 8);
+    return p;
+}
+
+struct BackwardPlan { uint32_t piece, splits; size_t ldx, ldg, ldp, x_off, g_off, p_off, bytes; };
+static BackwardPlan backward_plan(uint32_t rows, uint32_t docs, uint32_t dim, int sms) {
+    BackwardPlan p;
+    const uint32_t pairs = std::max(1, sms / 2);
+    const uint32_t mt = ceil_div(rows, 256), nd = ceil_div(dim, 256);
+    // documents per piece: G of about 128 MB, at least 2048 documents, whole rounds of tiles in the two large products
+    const uint64_t most = std::max<uint64_t>(8, (128ull << 20) / ((uint64_t)rows * 2) / kTileN);
+    uint32_t best = (uint32_t)std::min<uint64_t>(most, ceil_div(docs, kTileN));
+    p.piece = best * kTileN;
+    p.ldx = (dim + 7) / 8 * 8;
+    p.ldg = p.piece;
+    p.ldp = (dim + 3) / 4 * 4;
+    // dX contracts over the documents of a piece: few tiles and a long K, so K is split until every pair of SMs has a tile
+    const uint32_t kb = ceil_div(std::min(p.piece, docs), 64);
+    const uint32_t tiles = (rows <= 128 ? ceil_div(rows, 128) : mt) * nd, units = rows <= 128 ? (uint32_t)sms : pairs;
+    p.splits = std::max<uint32_t>(1, std::min<uint32_t>(units / std::max<uint32_t>(1, tiles), std::max<uint32_t>(1, kb / 8)));
+    p.x_off = 256;
+    p.g_off = p.x_off + round256((size_t)rows * p.ldx * 2);
+    p.p_off = p.g_off + round256((size_t)rows * p.ldg * 2);
+    p.bytes = p.p_off + round256((size_t)p.splits * rows * p.ldp * 4);
+    return p;
+}
+
+struct LossCall {
+    uint32_t rows, docs, dim;
+    const void *x, *w;
+    uint64_t ldx, ldw;
+    const uint32_t *target;
+    float scale;
+    int sms;
+    uint32_t *err;
+    cudaStream_t st;
+};
+
+template <class T, int CG>
+static int forward_run(const LossCall &c, const ForwardPlan &p, uint8_t *ws, float *loss, float *lse) {
+    using S = tile::Shape<Half16<T>::kind, CG, kTileN>;
+    float2 *part = reinterpret_cast<float2 *>(ws), *carry = reinterpret_cast<float2 *>(ws + p.part_bytes);
+    const Operand x{c.x, c.rows, c.dim, c.ldx};
+    for (uint32_t v0 = 0; v0 < c.docs; v0 += p.piece) {
+        const uint32_t n = std::min(p.piece, c.docs - v0);
+        const Operand w{static_cast<const T *>(c.w) + (size_t)v0 * c.ldw, n, c.dim, c.ldw};
+        LseEpi::Args ea{part, c.target, 2 * ceil_div(n, kTileN), c.rows, n, v0, c.scale * kLog2e};
+        AP_TRY((tile_launch<S, LseEpi>(x, w, c.rows, n, c.dim, 1, Scales{}, ea, c.sms, c.err, c.st)));
+        JoinArgs ja{part, carry, c.x, c.w, c.ldx, c.ldw, c.target, loss, lse, c.rows, c.docs, c.dim, ea.parts, v0 == 0 ? 1u : 0u,
+                    v0 + n == c.docs ? 1u : 0u, c.scale};
+        loss_join_kernel<T><<<ceil_div(c.rows, 8), 256, 0, c.st>>>(ja);
+        AP_CUDA(cudaGetLastError());
+    }
+    return AP_OK;
+}
+
+template <class T, int CG>
+static int backward_run(const LossCall &c, const BackwardPlan &p, uint8_t *ws, const float *loss, const float *lse, const float *grad, void *dx,
+                        uint64_t lddx, void *dw, uint64_t lddw) {
+    constexpr int KIND = Half16<T>::kind;
+    using SG = tile::Shape<KIND, CG, kTileN>;                       // G: rows x documents, over dim
+    using SX = tile::Shape<KIND, CG, kTileN, false, true>;          // dX: rows x dim, over documents
+    using SW = tile::Shape<KIND, 2, kTileN, true, true>;            // dW: documents x dim, over rows
+    float *factor = reinterpret_cast<float *>(ws);
+    T *xc = reinterpret_cast<T *>(ws + p.x_off), *g = reinterpret_cast<T *>(ws + p.g_off);
+    float *part = reinterpret_cast<float *>(ws + p.p_off);
+    PrepArgs pa{c.x, xc, c.ldx, p.ldx, c.target, grad, factor, c.rows, c.docs, c.dim, c.scale};
+    grad_prep_kernel<T><<<1 + std::min<uint32_t>(ceil_div(c.rows, 8), 4 * (uint32_t)c.sms), 256, 0, c.st>>>(pa);
+    AP_CUDA(cudaGetLastError());
+    const Operand x{xc, c.rows, c.dim, p.ldx};
+    for (uint32_t v0 = 0; v0 < c.docs; v0 += p.piece) {
+        const uint32_t n = std::min(p.piece, c.docs - v0);
+        const Operand w{static_cast<const T *>(c.w) + (size_t)v0 * c.ldw, n, c.dim, c.ldw};
+        const Operand go{g, c.rows, n, p.ldg};
+        typename GradEpi<T>::Args ga{};
+        ga.out.out = g; ga.out.ld = p.ldg; ga.out.m = c.rows; ga.out.n = n; ga.out.alpha = 1.f; ga.out.vec = 1;
+        ga.target = c.target; ga.loss = loss; ga.lse = lse; ga.grad = grad; ga.factor = factor; ga.col0 = v0; ga.docs = c.docs; ga.c = c.scale * kLog2e;
+        AP_TRY((tile_launch<SG, GradEpi<T>>(x, w, c.rows, n, c.dim, 1, Scales{}, ga, c.sms, c.err, c.st)));
+        typename StoreEpi<T>::Args wa{};
+        wa.out = static_cast<T *>(dw) + (size_t)v0 * lddw; wa.ld = lddw; wa.m = n; wa.n = c.dim; wa.alpha = 1.f; wa.alpha_dev = factor + 1;
+        wa.vec = aligned(wa.out, lddw * 2, 16);
+        AP_TRY((tile_launch<SW, StoreEpi<T>>(go, x, n, c.dim, c.rows, 1, Scales{}, wa, c.sms, c.err, c.st)));
+        typename StoreEpi<float>::Args xa{};
+        xa.out = part; xa.ld = p.ldp; xa.split_stride = (size_t)c.rows * p.ldp; xa.m = c.rows; xa.n = c.dim; xa.alpha = 1.f; xa.add = v0 != 0; xa.vec = 1;
+        const uint32_t kb = ceil_div(n, 64);
+        if (v0 != 0 && kb < p.splits) {
+            // a short last piece: fewer splits, the first of them
+            AP_TRY((tile_launch<SX, StoreEpi<float>>(go, w, c.rows, c.dim, n, 1, Scales{}, xa, c.sms, c.err, c.st)));
+        } else {
+            AP_TRY((tile_launch<SX, StoreEpi<float>>(go, w, c.rows, c.dim, n, p.splits, Scales{}, xa, c.sms, c.err, c.st)));
+        }
+    }
+    FinishArgs fa{part, factor, dx, p.ldp, lddx, c.rows, c.dim, p.splits};
+    const uint64_t quads = (uint64_t)c.rows * ((c.dim + 3) / 4);
+    grad_finish_kernel<T><<<(uint32_t)std::min<uint64_t>((quads + 255) / 256, 8ull * c.sms), 256, 0, c.st>>>(fa);
+    AP_CUDA(cudaGetLastError());
+    return AP_OK;
+}
+
+// ---- scores: the shapes ---------------------------------------------------------------------------------------------------
+template <class T, int CG, int N>
+static int scores_run(const ap_scaled_rows &a, const ap_scaled_rows &b, uint32_t dim, float alpha, T *out, uint64_t ldo, int sms, uint32_t *err,
+                      cudaStream_t st) {
+    using S = tile::Shape<tile::kE4m3, CG, N>;
+    const Operand oa{a.q, a.rows, dim, a.ldq}, ob{b.q, b.rows, dim, b.ldq};
+    typename StoreEpi<T>::Args ea{};
+    ea.out = out; ea.ld = ldo; ea.m = a.rows; ea.n = b.rows; ea.alpha = alpha; ea.vec = aligned(out, ldo * sizeof(T), 16);
+    const Scales sc{a.scale, b.scale, a.ld_scale, b.ld_scale, a.rows, b.rows};
+    return tile_launch<S, StoreEpi<T>>(oa, ob, a.rows, b.rows, dim, 1, sc, ea, sms, err, st);
+}
+template <class T>
+static int scores_pick(const ap_scaled_rows &a, const ap_scaled_rows &b, uint32_t dim, float alpha, void *out, uint64_t ldo, int sms, uint32_t *err,
+                       cudaStream_t st) {
+    T *o = static_cast<T *>(out);
+    if (a.rows > 128) return scores_run<T, 2, 224>(a, b, dim, alpha, o, ldo, sms, err, st);
+    // few rows: one CTA per tile, and narrow tiles while wide ones would leave SMs without any
+    if (ceil_div(b.rows, 224) >= (uint32_t)sms) return scores_run<T, 1, 224>(a, b, dim, alpha, o, ldo, sms, err, st);
+    return scores_run<T, 1, 64>(a, b, dim, alpha, o, ldo, sms, err, st);
+}
+
+static int check_loss(const char *what, uint32_t rows, uint32_t docs, uint32_t dim, uint32_t type, const void *x, uint64_t ldx, const void *w, uint64_t ldw,
+                      const uint32_t *target, float scale) {
+    if (!x || !w || !target) return fail(AP_ERR_ARG, "%s: null argument", what);
+    if (type != AP_TYPE_F16 && type != AP_TYPE_BF16) return fail(AP_ERR_ARG, "%s: type %u: the vectors are f16 or bf16", what, type);
+    if (rows == 0 || docs == 0 || dim == 0) return fail(AP_ERR_ARG, "%s: %u queries, %u documents, %u values: none may be 0", what, rows, docs, dim);
+    if (rows > (1u << 20) || docs > (1u << 30) || dim > (1u << 16))
+        return fail(AP_ERR_LIMIT, "%s: up to 2^20 queries, 2^30 documents, 2^16 values", what);
+    if (ldx < dim || ldw < dim) return fail(AP_ERR_ARG, "%s: a row stride is shorter than a row", what);
+    if (!aligned(x, ldx * 2, 16) || !aligned(w, ldw * 2, 16)) return fail(AP_ERR_ARG, "%s: rows start on 16-byte boundaries (base and stride)", what);
+    if (!std::isfinite(scale)) return fail(AP_ERR_ARG, "%s: the scale is not finite", what);
+    return AP_OK;
+}
+
+}  // namespace apoe
+
+using namespace apoe;
+
+extern "C" int ap_dense_check_status(int device, void *stream) {
+    DeviceScope scope;
+    AP_TRY(scope.enter(device));
+    cudaStream_t st = (cudaStream_t)stream;
+    uint32_t ew = 0;
+    AP_CUDA(cudaMemcpyFromSymbolAsync(&ew, dense_error_word, 4, 0, cudaMemcpyDeviceToHost, st));
+    AP_CUDA(cudaStreamSynchronize(st));
+    if (!ew) return AP_OK;
+    const uint32_t zero = 0;
+    AP_CUDA(cudaMemcpyToSymbolAsync(dense_error_word, &zero, 4, 0, cudaMemcpyHostToDevice, st));
+    AP_CUDA(cudaStreamSynchronize(st));
+    return fail(AP_ERR_DEVICE, "a dense operator raised error word %u (a bounded wait ran out)", ew);
+}
+
+extern "C" int ap_quantize_rows_device(int device, uint32_t rows, uint32_t dim, uint32_t type, const void *src, uint64_t ld, uint8_t *q, uint64_t ldq,
+                                       uint8_t *scale, uint64_t ld_scale, void *stream) {
+    const int size = elem_size(type);
+    if (!size) return fail(AP_ERR_ARG, "quantize: type %u", type);
+    if (dim == 0) return fail(AP_ERR_ARG, "quantize: rows of 0 values");
+    if (rows == 0) return AP_OK;
+    if (!src || !q || !scale) return fail(AP_ERR_ARG, "quantize: null argument");
+    const uint32_t blocks = ceil_div(dim, 128);
+    if (ld < dim || ldq < dim || ld_scale < blocks) return fail(AP_ERR_ARG, "quantize: a row stride is shorter than a row");
+    if ((uintptr_t)src % (uint32_t)size) return fail(AP_ERR_ARG, "quantize: the source is not aligned to its type");
+    DeviceScope scope;
+    AP_TRY(scope.enter(device));
+    int sms;
+    AP_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    QuantArgs a{src, q, scale, ld, ldq, ld_scale, (uint64_t)rows * blocks, dim, blocks, 0};
+    a.vec = aligned(src, ld * size, 4 * size) && aligned(q, ldq, 4);
+    const uint32_t grid = (uint32_t)std::min<uint64_t>((a.items + 8 * kQuantUnroll - 1) / (8 * kQuantUnroll), 8ull * sms);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (type == AP_TYPE_F32) quantize_kernel<float><<<grid, 256, 0, st>>>(a);
+    else if (type == AP_TYPE_F16) quantize_kernel<__half><<<grid, 256, 0, st>>>(a);
+    else quantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
+    AP_CUDA(cudaGetLastError());
+    return AP_OK;
+}
+
+extern "C" int ap_scaled_scores_device(int device, uint32_t dim, const ap_scaled_rows *a, const ap_scaled_rows *b, float alpha, uint32_t out_type, void *out,
+                                       uint64_t ldo, void *stream) {
+    if (!a || !b) return fail(AP_ERR_ARG, "scores: null argument");
+    const int size = elem_size(out_type);
+    if (!size) return fail(AP_ERR_ARG, "scores: output type %u", out_type);
+    if (dim == 0) return fail(AP_ERR_ARG, "scores: rows of 0 values");
+    if (a->rows == 0 || b->rows == 0) return AP_OK;
+    if (!a->q || !a->scale || !b->q || !b->scale || !out) return fail(AP_ERR_ARG, "scores: null argument");
+    if (a->rows > (1u << 30) || b->rows > (1u << 30) || dim > (1u << 20)) return fail(AP_ERR_LIMIT, "scores: up to 2^30 rows of 2^20 values");
+    const uint32_t blocks = ceil_div(dim, 128);
+    if (a->ldq < dim || b->ldq < dim || a->ld_scale < blocks || b->ld_scale < blocks || ldo < b->rows)
+        return fail(AP_ERR_ARG, "scores: a row stride is shorter than a row");
+    if (!aligned(a->q, a->ldq, 16) || !aligned(b->q, b->ldq, 16)) return fail(AP_ERR_ARG, "scores: 8-bit rows start on 16-byte boundaries (base and stride)");
+    if ((uintptr_t)out % (uint32_t)size) return fail(AP_ERR_ARG, "scores: the output is not aligned to its type");
+    if ((uint64_t)ceil_div(a->rows, 128) * ceil_div(b->rows, 64) >= (1ull << 32)) return fail(AP_ERR_LIMIT, "scores: %u x %u scores in one call", a->rows, b->rows);
+    DeviceScope scope;
+    AP_TRY(scope.enter(device));
+    int sms;
+    uint32_t *err;
+    AP_TRY(device_facts(device, &sms, &err));
+    cudaStream_t st = (cudaStream_t)stream;
+    if (out_type == AP_TYPE_F32) return scores_pick<float>(*a, *b, dim, alpha, out, ldo, sms, err, st);
+    if (out_type == AP_TYPE_F16) return scores_pick<__half>(*a, *b, dim, alpha, out, ldo, sms, err, st);
+    return scores_pick<__nv_bfloat16>(*a, *b, dim, alpha, out, ldo, sms, err, st);
+}
+
+extern "C" int ap_softmax_loss_workspace(int device, uint32_t rows, uint32_t docs, uint32_t dim, int backward, size_t *bytes) {
+    if (!bytes) return fail(AP_ERR_ARG, "softmax loss: null argument");
+    if (rows == 0 || docs == 0 || dim == 0) return fail(AP_ERR_ARG, "softmax loss: %u queries, %u documents, %u values: none may be 0", rows, docs, dim);
+    if (!backward) { *bytes = forward_plan(rows, docs).bytes; return AP_OK; }
+    int sms;
+    AP_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    *bytes = backward_plan(rows, docs, dim, sms).bytes;
+    return AP_OK;
+}
+
+extern "C" int ap_softmax_loss_forward_device(int device, uint32_t rows, uint32_t docs, uint32_t dim, uint32_t type, const void *queries, uint64_t ldq,
+                                              const void *documents, uint64_t ldd, const uint32_t *target, float scale, float *loss, float *lse,
+                                              void *workspace, size_t workspace_bytes, void *stream) {
+    AP_TRY(check_loss("softmax loss", rows, docs, dim, type, queries, ldq, documents, ldd, target, scale));
+    if (!loss || !lse || !workspace) return fail(AP_ERR_ARG, "softmax loss: null argument");
+    const ForwardPlan p = forward_plan(rows, docs);
+    if (workspace_bytes < p.bytes) return fail(AP_ERR_ARG, "softmax loss: the workspace has %zu bytes, %zu are needed", workspace_bytes, p.bytes);
+    if ((uintptr_t)workspace % 256) return fail(AP_ERR_ARG, "softmax loss: the workspace starts on a 256-byte boundary");
+    DeviceScope scope;
+    AP_TRY(scope.enter(device));
+    LossCall c{rows, docs, dim, queries, documents, ldq, ldd, target, scale, 0, nullptr, (cudaStream_t)stream};
+    AP_TRY(device_facts(device, &c.sms, &c.err));
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    if (type == AP_TYPE_F16) return rows <= 128 ? forward_run<__half, 1>(c, p, ws, loss, lse) : forward_run<__half, 2>(c, p, ws, loss, lse);
+    return rows <= 128 ? forward_run<__nv_bfloat16, 1>(c, p, ws, loss, lse) : forward_run<__nv_bfloat16, 2>(c, p, ws, loss, lse);
+}
+
+extern "C" int ap_softmax_loss_backward_device(int device, uint32_t rows, uint32_t docs, uint32_t dim, uint32_t type, const void *queries, uint64_t ldq,
+                                               const void *documents, uint64_t ldd, const uint32_t *target, float scale, const float *loss,
+                                               const float *lse, const float *grad_loss, void *grad_queries, uint64_t ldgq, void *grad_documents,
+                                               uint64_t ldgd, void *workspace, size_t workspace_bytes, void *stream) {
+    AP_TRY(check_loss("softmax loss gradient", rows, docs, dim, type, queries, ldq, documents, ldd, target, scale));
+    if (!loss || !lse || !grad_loss || !grad_queries || !grad_documents || !workspace) return fail(AP_ERR_ARG, "softmax loss gradient: null argument");
+    if (ldgq < dim || ldgd < dim) return fail(AP_ERR_ARG, "softmax loss gradient: a row stride is shorter than a row");
+    if (!aligned(grad_queries, ldgq * 2, 8) || (uintptr_t)grad_documents % 2) return fail(AP_ERR_ARG, "softmax loss gradient: rows of the queries' gradient start on 8-byte boundaries");
+    DeviceScope scope;
+    AP_TRY(scope.enter(device));
+    LossCall c{rows, docs, dim, queries, documents, ldq, ldd, target, scale, 0, nullptr, (cudaStream_t)stream};
+    AP_TRY(device_facts(device, &c.sms, &c.err));
+    const BackwardPlan p = backward_plan(rows, docs, dim, c.sms);
+    if (workspace_bytes < p.bytes) return fail(AP_ERR_ARG, "softmax loss gradient: the workspace has %zu bytes, %zu are needed", workspace_bytes, p.bytes);
+    if ((uintptr_t)workspace % 256) return fail(AP_ERR_ARG, "softmax loss gradient: the workspace starts on a 256-byte boundary");
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    if (type == AP_TYPE_F16)
+        return rows <= 128 ? backward_run<__half, 1>(c, p, ws, loss, lse, grad_loss, grad_queries, ldgq, grad_documents, ldgd)
+                           : backward_run<__half, 2>(c, p, ws, loss, lse, grad_loss, grad_queries, ldgq, grad_documents, ldgd);
+    return rows <= 128 ? backward_run<__nv_bfloat16, 1>(c, p, ws, loss, lse, grad_loss, grad_queries, ldgq, grad_documents, ldgd)
+                       : backward_run<__nv_bfloat16, 2>(c, p, ws, loss, lse, grad_loss, grad_queries, ldgq, grad_documents, ldgd);
+}

@@ -29,7 +29,7 @@
 #include <cstdio>
 #include <mutex>
 
-#include "apoe_common.cuh"
+#include "apoe_tile.cuh"
 
 extern "C" int ap_merge_shard_keys(int device, uint32_t shards, uint32_t nq, uint32_t per_shard, const unsigned long long *keys,
                                    uint32_t top_k, uint32_t *out_ids, float *out_dis, void *stream);
@@ -484,11 +484,7 @@ __global__ void __launch_bounds__(kExThreads, 1) exact_dense_topk_kernel(const _
 // ---------------------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static int encode_fn(EncodeTiledFn *out) {
+int encode_fn(EncodeTiledFn *out) {
     static std::mutex mu;
     static EncodeTiledFn cached = nullptr;
     std::lock_guard<std::mutex> lock(mu);

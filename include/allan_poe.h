@@ -340,6 +340,61 @@ int ap_exact_topk_device(ap_index *ix, const ap_queries *q, float sparse_weight,
                          uint32_t flags, uint32_t top_k, uint32_t *out_ids, float *out_dis, void *stream, ap_exact_stats *stats);
 int ap_exact_release(ap_index *ix);
 
+/* ---- dense operators -------------------------------------------------------------------------------------- */
+/* Operators over the vectors a dense encoder makes of queries and documents: 8-bit rows and their scores, and the loss the
+ * encoder is trained with.  No counterpart in the reference.  Every pointer is device memory of `device`; rows may be further
+ * apart than they are long (strides in values).  The calls only enqueue work on `stream` (a cudaStream_t), keep no state
+ * between calls, allocate nothing, leave the caller's current device as it was and may be captured into a graph.  Calls that
+ * overlap need outputs and workspaces of their own.  Results do not depend on timing: the same call gives the same bits. */
+#define AP_TYPE_F32 0u
+#define AP_TYPE_F16 1u
+#define AP_TYPE_BF16 2u
+/* Waits for `stream` and reports (and clears) the device's error word: AP_ERR_DEVICE when a bounded wait of an earlier dense
+ * operator ran out (its outputs are then incomplete), else AP_OK. */
+int ap_dense_check_status(int device, void *stream);
+
+/* Rows in 8 bits: for each block of 128 values (the last one of a row may be shorter) e is the smallest integer >= -126 with
+ * max |x| <= 448 * 2^e, q = e4m3(x * 2^-e) to nearest even, scale byte = e + 127 (value 2^e).  A NaN becomes the e4m3 NaN and
+ * does not count for the maximum; an infinity becomes +-448 with a scale whose product overflows to infinity in fp32.
+ * src: rows x dim values of `type`, ld apart; q: bytes, ldq apart; scale: ceil(dim / 128) bytes per row, ld_scale apart.
+ * rows = 0 does nothing. */
+int ap_quantize_rows_device(int device, uint32_t rows, uint32_t dim, uint32_t type, const void *src, uint64_t ld, uint8_t *q,
+                            uint64_t ldq, uint8_t *scale, uint64_t ld_scale, void *stream);
+typedef struct {
+    uint32_t rows;
+    const uint8_t *q;      /* e4m3, rows on 16-byte boundaries */
+    uint64_t ldq;          /* bytes, a multiple of 16 */
+    const uint8_t *scale;  /* byte s stands for 2^(s - 127), s < 255; ceil(dim / 128) per row */
+    uint64_t ld_scale;
+} ap_scaled_rows;
+/* Scores of such rows: out[i][j] = alpha * sum over blocks of scale_a * scale_b * <a, b>, summed in fp32 and rounded once to
+ * out_type.  out: a->rows x b->rows, ldo values apart.  No rows on either side: does nothing. */
+int ap_scaled_scores_device(int device, uint32_t dim, const ap_scaled_rows *a, const ap_scaled_rows *b, float alpha,
+                            uint32_t out_type, void *out, uint64_t ldo, void *stream);
+
+/* Softmax loss of queries over documents (the contrastive loss of a dense encoder: one document per query is its target, all
+ * others are negatives), without holding the rows x docs matrix:
+ *   l[t][v] = scale * <query t, document v>,  lse[t] = log sum_v exp l[t][v],  loss[t] = lse[t] - l[t][target[t]].
+ * queries, documents: f16 or bf16, rows on 16-byte boundaries (base and stride), row strides ldq / ldd in values.
+ * target: document ids; 0xFFFFFFFF = the row takes no part (loss and lse 0, gradient 0, whatever its vector holds); any
+ * other id >= docs gives NaN in loss and lse and no gradient.
+ * The backward call takes loss and lse as the forward call on the same inputs wrote them and the gradient of each row's
+ * loss, and writes the gradients of both sides (type of the vectors):
+ *   G[t][v] = grad_loss[t] * (exp(l[t][v] - lse[t]) - [v = target[t]]),  grad_queries = scale * G * documents,
+ *   grad_documents = scale * G^T * queries.
+ * Rows of grad_queries start on 8-byte boundaries.  workspace: device memory on a 256-byte boundary, at least as many bytes as
+ * ap_softmax_loss_workspace gives for the call (backward = 0 or 1); its contents mean nothing before or after.
+ * At least one query, document and value; at most 2^20, 2^30 and 2^16. */
+int ap_softmax_loss_workspace(int device, uint32_t rows, uint32_t docs, uint32_t dim, int backward, size_t *bytes);
+int ap_softmax_loss_forward_device(int device, uint32_t rows, uint32_t docs, uint32_t dim, uint32_t type, const void *queries,
+                                   uint64_t ldq, const void *documents, uint64_t ldd, const uint32_t *target, float scale,
+                                   float *loss, float *lse, void *workspace, size_t workspace_bytes, void *stream);
+int ap_softmax_loss_backward_device(int device, uint32_t rows, uint32_t docs, uint32_t dim, uint32_t type, const void *queries,
+                                    uint64_t ldq, const void *documents, uint64_t ldd, const uint32_t *target, float scale,
+                                    const float *loss, const float *lse, const float *grad_loss, void *grad_queries,
+                                    uint64_t ldgq, void *grad_documents, uint64_t ldgd, void *workspace,
+                                    size_t workspace_bytes, void *stream);
+
 /* ---- corpus-sharded search ------------------------------------------------------------------------------ */
 /* No counterpart in the reference (one GPU, one index).  Documents [start, start + count) of an n-document corpus belong to
  * shard `shard` of `shards`: contiguous ranges whose sizes differ by at most one. */
