@@ -146,83 +146,83 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantArgs a) {
 // ---------------------------------------------------------------------------------------------------------------------
 // epilogues of the tile engine
 // ---------------------------------------------------------------------------------------------------------------------
-// Stores a tile: 32 columns at a time through the warp's 4 KB of shared memory (16-byte units exchanged by row so neither
-// side has bank conflicts), then whole 128-byte (f32) or 64-byte (f16, bf16) pieces of rows.
+// Stores a tile through the warp's 4 KB of shared memory, in boxes of 32 rows x 64 bytes (16-byte units exchanged as the
+// 64-byte TMA swizzle does, so writing them has no bank conflicts).  Two boxes are in flight: one leaves by TMA while the next
+// is written; the tensor map cuts off rows that lie outside, but columns only by 16 bytes.  So the last columns of a row that
+// ends inside a box, and all of an output whose rows do not start on 16-byte boundaries, are written element by element.
 template <class T>
 struct StoreEpi {
     struct Args {
-        T *out;
-        size_t ld, split_stride;     // elements; result of split s starts at out + s * split_stride
+        T *out;                      // results of the splits: stack of m x n matrices, only the first one without `tma`
+        size_t ld;                   // elements
         uint32_t m, n;
         float alpha;
         const float *alpha_dev;      // another factor, read on the device (may be null)
-        uint32_t add;                // f32 only: add to what is there
-        uint32_t vec;                // rows of `out` start on 16-byte boundaries
+        uint32_t add;                // f32 with `tma` only: add to what is there
+        uint32_t tma;
+        uint32_t padded;             // what follows a row up to the next 16 bytes may be overwritten
     };
+    static constexpr int UNITS = (int)sizeof(T) / 2;       // boxes of 32 columns
+    static constexpr int COLS = 32 / UNITS;                // columns of a box
     const Args &a;
     uint8_t *st;
+    const CUtensorMap *map;
     int lane;
     float alpha;
-    uint32_t row0 = 0;
-    T *base = nullptr;
-    __device__ __forceinline__ StoreEpi(const Args &args, uint8_t *staging, int lane_) : a(args), st(staging), lane(lane_) {
+    uint32_t row0 = 0, split = 0, boxes = 0;
+    __device__ __forceinline__ StoreEpi(const Args &args, uint8_t *staging, const CUtensorMap *out, int lane_) : a(args), st(staging), map(out), lane(lane_) {
         alpha = a.alpha_dev ? a.alpha * __ldg(a.alpha_dev) : a.alpha;
     }
-    __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t split, uint32_t) { row0 = r0; base = a.out + split * a.split_stride; }
+    __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t s, uint32_t) { row0 = r0; split = s; }
     __device__ __forceinline__ void end() {}
+    __device__ __forceinline__ void finish() { if (lane == 0) tile::store_wait_all(); }
     __device__ __forceinline__ void chunk(uint32_t (&r)[32], uint32_t col) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
         put(r, col);
     }
     __device__ __forceinline__ void put(const uint32_t (&r)[32], uint32_t col) {
-        if (row0 >= a.m || col >= a.n) return;          // uniform over the warp
-        const uint32_t rows = min(32u, a.m - row0), cols = min(32u, a.n - col);
-        if constexpr (sizeof(T) == 4) {
+        if (row0 >= a.m) return;                           // uniform over the warp, as all conditions but the lane's own
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<uint4 *>(st + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-        } else {
+        for (int u = 0; u < UNITS; ++u) {
+            const uint32_t c = col + u * COLS;
+            if (c >= a.n) return;
+            uint8_t *box = st + (boxes & 1) * 2048;
+            if (boxes >= 2) {                              // the box written two rounds ago has left
+                if (lane == 0) tile::store_wait_read<1>();
+                __syncwarp();
+            }
+            ++boxes;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t p[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = Half16<T>::pack(__uint_as_float(r[8 * j + 2 * i]), __uint_as_float(r[8 * j + 2 * i + 1]));
-                *reinterpret_cast<uint4 *>(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
-            }
-        }
-        __syncwarp();
-        constexpr int UNITS = (int)sizeof(T) * 2;       // 16-byte units of a row's 32 columns
-        constexpr int RPI = 32 / UNITS;                 // rows per pass
-        if (a.vec && cols == 32) {
-#pragma unroll
-            for (int i = 0; i < 32 / RPI; ++i) {
-                const int row = i * RPI + lane / UNITS, j = lane % UNITS;
-                const int sw = sizeof(T) == 4 ? (j ^ (row & 7)) : (j ^ ((row >> 1) & 3));
-                uint4 v = *reinterpret_cast<const uint4 *>(st + row * (UNITS * 16) + (sw << 4));
-                if ((uint32_t)row < rows) {
-                    uint4 *o = reinterpret_cast<uint4 *>(base + (size_t)(row0 + row) * a.ld + col) + j;
-                    if constexpr (sizeof(T) == 4) {
-                        if (a.add) {
-                            const float4 w = *reinterpret_cast<const float4 *>(o);
-                            v.x = __float_as_uint(__uint_as_float(v.x) + w.x); v.y = __float_as_uint(__uint_as_float(v.y) + w.y);
-                            v.z = __float_as_uint(__uint_as_float(v.z) + w.z); v.w = __float_as_uint(__uint_as_float(v.w) + w.w);
-                        }
-                    }
-                    *o = v;
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (sizeof(T) == 4) p[i] = r[16 * u + 4 * j + i];
+                    else p[i] = Half16<T>::pack(__uint_as_float(r[8 * j + 2 * i]), __uint_as_float(r[8 * j + 2 * i + 1]));
                 }
+                *reinterpret_cast<uint4 *>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
             }
-        } else if ((uint32_t)lane < cols) {
-            for (uint32_t row = 0; row < rows; ++row) {
-                constexpr int PER = 16 / (int)sizeof(T);
-                const int j = lane / PER, sw = sizeof(T) == 4 ? (j ^ ((int)row & 7)) : (j ^ (((int)row >> 1) & 3));
-                T v = *reinterpret_cast<const T *>(st + row * (UNITS * 16) + (sw << 4) + (lane % PER) * sizeof(T));
-                T *o = base + (size_t)(row0 + row) * a.ld + col + lane;
-                if constexpr (sizeof(T) == 4) { if (a.add) v += *o; }
-                *o = v;
+            if (a.tma && (a.padded || c + COLS <= a.n)) {
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    if (sizeof(T) == 4 && a.add) tile::add_3d(map, box, (int)c, (int)row0, (int)split);
+                    else tile::store_3d(map, box, (int)c, (int)row0, (int)split);
+                    tile::store_commit();
+                }
+            } else {
+                __syncwarp();
+                const uint32_t rows = min(32u, a.m - row0);
+                constexpr int PER = 16 / (int)sizeof(T), RPI = 32 / COLS;      // values of a unit, rows a pass covers
+                const int k = lane % COLS;
+                if (c + k < a.n)
+                    for (uint32_t row = lane / COLS; row < rows; row += RPI)
+                        a.out[(size_t)(row0 + row) * a.ld + c + k] =
+                            *reinterpret_cast<const T *>(box + row * 64 + (((k / PER) ^ ((row >> 1) & 3)) << 4) + (k % PER) * sizeof(T));
+                __syncwarp();
             }
         }
-        __syncwarp();
     }
 };
 
@@ -245,14 +245,14 @@ struct LseEpi {
     int lane;
     uint32_t row = 0, part = 0, tgt = 0;
     float top = 0.f, sum = 0.f;
-    __device__ __forceinline__ LseEpi(const Args &args, uint8_t *, int lane_) : a(args), lane(lane_) {}
+    __device__ __forceinline__ LseEpi(const Args &args, uint8_t *, const CUtensorMap *, int lane_) : a(args), lane(lane_) {}
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t, uint32_t p) {
         row = r0 + lane; part = p;
         tgt = row < a.m ? __ldg(a.target + row) - a.col0 : kNoTarget;   // columns are below 2^31: no match for a target of another piece
         top = -1.0e30f; sum = 0.f;
     }
     __device__ __forceinline__ void chunk(uint32_t (&r)[32], uint32_t col) {
-        float v[32], m = top;
+        float v[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * a.c;
         const uint32_t at = tgt - col, cols = a.n > col ? a.n - col : 0u;
@@ -260,13 +260,18 @@ struct LseEpi {
 #pragma unroll
             for (int j = 0; j < 32; ++j) if (at == (uint32_t)j || (uint32_t)j >= cols) v[j] = -INFINITY;
         }
+        // four chains each for the maximum and the sum: one would make the warp wait for its own last result 32 times over
+        float m4[4] = {top, v[1], v[2], v[3]}, s4[4] = {0.f, 0.f, 0.f, 0.f};
+        m4[0] = fmaxf(top, v[0]);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) m = fmaxf(m, v[j]);
-        float s0 = sum * exp2_fast(top - m), s1 = 0.f;
+        for (int j = 4; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
+        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) { s0 += exp2_fast(v[j] - m); s1 += exp2_fast(v[j + 1] - m); }
-        top = m; sum = s0 + s1;
+        for (int j = 0; j < 32; ++j) s4[j & 3] += exp2_fast(v[j] - m);
+        sum = sum * exp2_fast(top - m) + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+        top = m;
     }
+    __device__ __forceinline__ void finish() {}
     __device__ __forceinline__ void end() { if (row < a.m) a.part[(size_t)row * a.parts + part] = make_float2(top, sum); }
 };
 
@@ -286,7 +291,7 @@ struct GradEpi {
     StoreEpi<T> store;
     uint32_t tgt = 0;
     float lse2 = 0.f, g = 0.f, at_target = 0.f;
-    __device__ __forceinline__ GradEpi(const Args &args, uint8_t *staging, int lane) : a(args), store(args.out, staging, lane) {}
+    __device__ __forceinline__ GradEpi(const Args &args, uint8_t *staging, const CUtensorMap *out, int lane) : a(args), store(args.out, staging, out, lane) {}
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t n0, uint32_t s, uint32_t p) {
         store.begin(r0, n0, s, p);
         const uint32_t row = r0 + store.lane;
@@ -300,6 +305,7 @@ struct GradEpi {
         } else tgt = kNoTarget;
     }
     __device__ __forceinline__ void end() {}
+    __device__ __forceinline__ void finish() { store.finish(); }
     __device__ __forceinline__ void chunk(uint32_t (&r)[32], uint32_t col) {
         const bool live = g != 0.f;      // rows without a target may hold anything, NaN included: their G is zero
 #pragma unroll
@@ -475,25 +481,51 @@ static int make_map_2d(CUtensorMap *map, int kind, const void *base, uint64_t ro
     if (r != CUDA_SUCCESS) return fail(AP_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
     return AP_OK;
 }
+// a stack of m x n results, written in boxes of 32 rows x 64 bytes
+static int make_map_out(CUtensorMap *map, CUtensorMapDataType t, uint32_t size, void *base, uint64_t stack, uint64_t m, uint64_t n, uint64_t ld) {
+    EncodeTiledFn fn;
+    AP_TRY(encode_fn(&fn));
+    const cuuint64_t dims[3] = {n, m, stack};
+    const cuuint64_t strides[2] = {ld * size, m * ld * size};
+    const cuuint32_t box[3] = {64 / size, 32, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, t, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(AP_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+    return AP_OK;
+}
+template <class T> struct MapType;
+template <> struct MapType<float> { static constexpr CUtensorMapDataType v = CU_TENSOR_MAP_DATA_TYPE_FLOAT32; };
+template <> struct MapType<__half> { static constexpr CUtensorMapDataType v = CU_TENSOR_MAP_DATA_TYPE_FLOAT16; };
+template <> struct MapType<__nv_bfloat16> { static constexpr CUtensorMapDataType v = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; };
+template <class T>
+static int out_map(CUtensorMap *map, const typename StoreEpi<T>::Args &a, uint32_t stack) {
+    return a.tma ? make_map_out(map, MapType<T>::v, sizeof(T), a.out, stack, a.m, a.n, a.ld) : AP_OK;
+}
+template <class T> static int out_map_of(CUtensorMap *map, const typename StoreEpi<T>::Args &a, uint32_t stack, const StoreEpi<T> *) { return out_map<T>(map, a, stack); }
+template <class T> static int out_map_of(CUtensorMap *map, const typename GradEpi<T>::Args &a, uint32_t, const GradEpi<T> *) { return out_map<T>(map, a.out, 1); }
+static int out_map_of(CUtensorMap *, const LseEpi::Args &, uint32_t, const LseEpi *) { return AP_OK; }
+
 struct Operand {   // a stored matrix: rows x cols, row stride in values
     const void *base;
     uint64_t rows, cols, ld;
 };
 static uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
-// C[m][n] = sum over k of A B^T on one shape.  K-major operands are stored rows x K, MN-major ones K x rows.
+// C[m][n] = sum over k of A B^T on one shape, K cut into at most `splits` parts.  K-major operands are stored rows x K, MN-major ones K x rows.
 template <class S, class Epi>
 static int tile_launch(const Operand &a, const Operand &b, uint32_t m, uint32_t n, uint32_t k, uint32_t splits, const Scales &sc,
                        const typename Epi::Args &epi, int sms, uint32_t *err, cudaStream_t st) {
-    CUtensorMap ma, mb;
+    CUtensorMap ma, mb, mo = {};
     AP_TRY(make_map_2d(&ma, S::KIND, a.base, a.rows, a.cols, a.ld, S::AMN ? 64 : 128));
     AP_TRY(make_map_2d(&mb, S::KIND, b.base, b.rows, b.cols, b.ld, S::BMN ? 64 : S::BR));
     Grid g;
     g.tiles_m = ceil_div(m, S::M);
     g.tiles_n = ceil_div(n, S::N);
-    g.splits = splits;
     g.kblocks = ceil_div(k, S::K);
-    g.total = g.tiles_m * g.tiles_n * splits;
+    g.kper = ceil_div(g.kblocks, splits);
+    g.total = g.tiles_m * g.tiles_n * ceil_div(g.kblocks, g.kper);
+    AP_TRY(out_map_of(&mo, epi, ceil_div(g.kblocks, g.kper), static_cast<const Epi *>(nullptr)));
     // row tiles that walk the columns together: all of them while their operand stays in L2 (32 MB of it), else 8
     const uint64_t row_bytes = (uint64_t)S::M * k * (S::SCALED ? 1 : 2);
     g.group_m = std::min<uint32_t>(g.tiles_m, (uint32_t)std::max<uint64_t>(8, (32ull << 20) / row_bytes));
@@ -508,7 +540,7 @@ static int tile_launch(const Operand &a, const Operand &b, uint32_t m, uint32_t 
     attr[0].val.clusterDim.x = S::CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    AP_CUDA(cudaLaunchKernelEx(&cfg, tile::tile_kernel<S, Epi>, ma, mb, g, sc, epi, err));
+    AP_CUDA(cudaLaunchKernelEx(&cfg, tile::tile_kernel<S, Epi>, ma, mb, mo, g, sc, epi, err));
     return AP_OK;
 }
 
@@ -553,7 +585,8 @@ static BackwardPlan backward_plan(uint32_t rows, uint32_t docs, uint32_t dim, in
     // dX contracts over the documents of a piece: few tiles and a long K, so K is split until every pair of SMs has a tile
     const uint32_t kb = ceil_div(std::min(p.piece, docs), 64);
     const uint32_t tiles = (rows <= 128 ? ceil_div(rows, 128) : mt) * nd, units = rows <= 128 ? (uint32_t)sms : pairs;
-    p.splits = std::max<uint32_t>(1, std::min<uint32_t>(units / std::max<uint32_t>(1, tiles), std::max<uint32_t>(1, kb / 8)));
+    p.splits = std::max<uint32_t>(1, std::min<uint32_t>(units / tiles, kb / 8));
+    p.splits = ceil_div(kb, ceil_div(kb, p.splits));
     p.x_off = 256;
     p.g_off = p.x_off + round256((size_t)rows * p.ldx * 2);
     p.p_off = p.g_off + round256((size_t)rows * p.ldg * 2);
@@ -609,22 +642,18 @@ static int backward_run(const LossCall &c, const BackwardPlan &p, uint8_t *ws, c
         const Operand w{static_cast<const T *>(c.w) + (size_t)v0 * c.ldw, n, c.dim, c.ldw};
         const Operand go{g, c.rows, n, p.ldg};
         typename GradEpi<T>::Args ga{};
-        ga.out.out = g; ga.out.ld = p.ldg; ga.out.m = c.rows; ga.out.n = n; ga.out.alpha = 1.f; ga.out.vec = 1;
+        ga.out.out = g; ga.out.ld = p.ldg; ga.out.m = c.rows; ga.out.n = n; ga.out.alpha = 1.f; ga.out.tma = 1; ga.out.padded = 1;
         ga.target = c.target; ga.loss = loss; ga.lse = lse; ga.grad = grad; ga.factor = factor; ga.col0 = v0; ga.docs = c.docs; ga.c = c.scale * kLog2e;
         AP_TRY((tile_launch<SG, GradEpi<T>>(x, w, c.rows, n, c.dim, 1, Scales{}, ga, c.sms, c.err, c.st)));
         typename StoreEpi<T>::Args wa{};
         wa.out = static_cast<T *>(dw) + (size_t)v0 * lddw; wa.ld = lddw; wa.m = n; wa.n = c.dim; wa.alpha = 1.f; wa.alpha_dev = factor + 1;
-        wa.vec = aligned(wa.out, lddw * 2, 16);
+        wa.tma = aligned(wa.out, lddw * 2, 16);
         AP_TRY((tile_launch<SW, StoreEpi<T>>(go, x, n, c.dim, c.rows, 1, Scales{}, wa, c.sms, c.err, c.st)));
         typename StoreEpi<float>::Args xa{};
-        xa.out = part; xa.ld = p.ldp; xa.split_stride = (size_t)c.rows * p.ldp; xa.m = c.rows; xa.n = c.dim; xa.alpha = 1.f; xa.add = v0 != 0; xa.vec = 1;
-        const uint32_t kb = ceil_div(n, 64);
-        if (v0 != 0 && kb < p.splits) {
-            // a short last piece: fewer splits, the first of them
-            AP_TRY((tile_launch<SX, StoreEpi<float>>(go, w, c.rows, c.dim, n, 1, Scales{}, xa, c.sms, c.err, c.st)));
-        } else {
-            AP_TRY((tile_launch<SX, StoreEpi<float>>(go, w, c.rows, c.dim, n, p.splits, Scales{}, xa, c.sms, c.err, c.st)));
-        }
+        xa.out = part; xa.ld = p.ldp; xa.m = c.rows; xa.n = c.dim; xa.alpha = 1.f; xa.add = v0 != 0; xa.tma = 1; xa.padded = 1;
+        // a short last piece has fewer splits, the first of them; without enough K blocks for each, one
+        const uint32_t splits = ceil_div(n, 64) < p.splits ? 1 : p.splits;
+        AP_TRY((tile_launch<SX, StoreEpi<float>>(go, w, c.rows, c.dim, n, splits, Scales{}, xa, c.sms, c.err, c.st)));
     }
     FinishArgs fa{part, factor, dx, p.ldp, lddx, c.rows, c.dim, p.splits};
     const uint64_t quads = (uint64_t)c.rows * ((c.dim + 3) / 4);
@@ -640,8 +669,9 @@ static int scores_run(const ap_scaled_rows &a, const ap_scaled_rows &b, uint32_t
     using S = tile::Shape<tile::kE4m3, CG, N>;
     const Operand oa{a.q, a.rows, dim, a.ldq}, ob{b.q, b.rows, dim, b.ldq};
     typename StoreEpi<T>::Args ea{};
-    ea.out = out; ea.ld = ldo; ea.m = a.rows; ea.n = b.rows; ea.alpha = alpha; ea.vec = aligned(out, ldo * sizeof(T), 16);
-    const Scales sc{a.scale, b.scale, a.ld_scale, b.ld_scale, a.rows, b.rows};
+    ea.out = out; ea.ld = ldo; ea.m = a.rows; ea.n = b.rows; ea.alpha = alpha; ea.tma = aligned(out, ldo * sizeof(T), 16);
+    const Scales sc{a.scale, b.scale, a.ld_scale, b.ld_scale, a.rows, b.rows,
+                    aligned(a.scale, a.ld_scale, 4) && aligned(b.scale, b.ld_scale, 4)};
     return tile_launch<S, StoreEpi<T>>(oa, ob, a.rows, b.rows, dim, 1, sc, ea, sms, err, st);
 }
 template <class T>

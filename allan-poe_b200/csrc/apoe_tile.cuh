@@ -44,36 +44,36 @@ struct Shape {
     static constexpr int K = SCALED ? 128 : 64;            // values of K in a stage: one 128-byte span
     static constexpr int BR = N / CG;                      // rows of B a CTA loads
     static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BR * 128;
-    static constexpr uint32_t SFA_BYTES = SCALED ? 512 : 0, SFB_BYTES = SCALED ? 1024 : 0;   // 128 and 256 scale words
-    static constexpr uint32_t LOAD_BYTES = A_BYTES + B_BYTES;
-    static constexpr uint32_t STAGE_BYTES = (LOAD_BYTES + SFA_BYTES + SFB_BYTES + 1023) / 1024 * 1024;
+    static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr uint32_t EPI_BYTES = kEpiWarps * 4096;
-    // as many stages as fit beside the epilogue's staging; e4m3: also one set of scale columns in tensor memory per stage
-    static constexpr int FIT = (int)((232448 - 1024 - 512 - EPI_BYTES) / STAGE_BYTES);
-    static constexpr int SF_COLS = SCALED ? 12 : 0;        // 4 (128 rows of A) + 8 (up to 256 rows of B)
-    static constexpr int SF_FIT = SCALED ? (512 - 2 * N) / 12 : 16;
-    static constexpr int STAGES = FIT < SF_FIT ? (FIT < 8 ? FIT : 8) : (SF_FIT < 8 ? SF_FIT : 8);
-    static constexpr uint32_t SMEM = STAGES * STAGE_BYTES + EPI_BYTES + 1024;
+    // scale words (e4m3): four K blocks at a time, 128 rows of A and up to 256 of B, in a ring of their own; each slot has its
+    // 12 columns of tensor memory
+    static constexpr int SF_SLOTS = SCALED ? 4 : 0;
+    static constexpr uint32_t SF_BYTES = SCALED ? 1536 : 0;
+    static constexpr uint32_t SF_ROOM = SF_SLOTS * SF_BYTES;
+    static constexpr int FIT = (int)((232448 - 1024 - 1024 - EPI_BYTES - SF_ROOM) / STAGE_BYTES);   // alignment, barriers, staging
+    static constexpr int STAGES = FIT < 8 ? FIT : 8;
+    static constexpr uint32_t SMEM = STAGES * STAGE_BYTES + SF_ROOM + EPI_BYTES + 1024;
     static_assert(STAGES >= 3, "too few stages");
-    static_assert(2 * N + STAGES * SF_COLS <= 512, "tensor memory");
+    static_assert(2 * N + SF_SLOTS * 12 <= 512, "tensor memory");
     static_assert(BR % 8 == 0 && (!BMN || BR % 64 == 0), "rows of B per CTA");
     static_assert(!SCALED || (!AMN && !BMN), "8-bit operands are K-major");
     static_assert(N % 32 == 0 && N <= 256, "columns");
     // kind::f16: D fp32 (bit 4), A / B type (bits 7, 10), MN-major flags (15, 16), N >> 3 (17), M >> 4 (24);
-    // kind::mxf8f6f4: e4m3 types are 0, scale type ue8m0 (bit 23), scale byte 0 of each word (bits 4, 29)
+    // kind::mxf8f6f4: e4m3 types are 0, scale type ue8m0 (bit 23), the byte of the scale words to use (bits 4 and 29: added)
     static constexpr uint32_t IDESC = SCALED ? ((1u << 23) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24))
                                              : ((1u << 4) | ((uint32_t)KIND << 7) | ((uint32_t)KIND << 10) | ((AMN ? 1u : 0u) << 15) |
                                                 ((BMN ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24));
 };
 
 // The tiles of one product and their order.  Groups of `group_m` row tiles walk the column tiles together, so the tiles in
-// flight share both operands in L2.  `splits` cuts K: split s contracts its share of the K blocks into a result of its own.
+// flight share both operands in L2.  K may be cut: split s contracts K blocks s * kper .. into a result of its own.
 struct Grid {
-    uint32_t tiles_m, tiles_n, splits, group_m, kblocks, total;
+    uint32_t tiles_m, tiles_n, group_m, kblocks, kper, total;   // kper: K blocks of a split (the last one may have fewer)
 };
 __device__ __forceinline__ void locate(const Grid &g, uint32_t id, uint32_t &mi, uint32_t &ni, uint32_t &si) {
     const uint32_t per = g.tiles_m * g.tiles_n;
-    si = id / per;
+    si = g.kper < g.kblocks ? id / per : 0u;
     id -= si * per;
     const uint32_t span = g.group_m * g.tiles_n, grp = id / span, r = id - grp * span;
     const uint32_t rows = min(g.group_m, g.tiles_m - grp * g.group_m);
@@ -97,20 +97,37 @@ __device__ __forceinline__ uint32_t leader_addr(const void *p) {   // shared::cl
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
     return a;
 }
-__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
+// Arrival on a barrier of the pair's leader.  With cluster-scope release: orders this thread's ordinary writes (the scale words)
+// for the other CTA.  Without: for arrivals that only say "read"; a release at cluster scope would first wait for the
+// epilogue's global stores, about a microsecond per tile.
+__device__ __forceinline__ void arrive_cluster_release(uint32_t addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-// waits with cluster-scope acquire: the arrivals may come from the pair's other CTA
+__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// Bounded waits; the second form sees what the pair's other CTA wrote before its releasing arrival.
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code, uint32_t limit = kWaitLimit) {
-    for (uint32_t i = 0; i < limit; ++i) {
+    for (uint32_t i = 0; i < limit; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    if (err) atomicExch(err, code);
+    return false;
+}
+__device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
+    for (uint32_t i = 0; i < kWaitLimit; ++i) {
         uint32_t ok;
         asm volatile("{\n\t.reg .pred p;\n\t"
                      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
                      "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
         if (ok) return true;
     }
-    if (err) atomicExch(err, code);
+    atomicExch(err, code);
     return false;
+}
+__device__ __forceinline__ bool elect_one() {   // true in one lane of the (whole) warp
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
 }
 template <int CG>
 __device__ __forceinline__ void load_2d(void *dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
@@ -167,6 +184,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t (&r)[32], uint32_t addr) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// One 64-byte wide box of shared memory to a matrix of a stack of them, plain or added to what is there (f32, in L2).
+__device__ __forceinline__ void store_3d(const CUtensorMap *map, const void *src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                 ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(src)) : "memory");
+}
+__device__ __forceinline__ void add_3d(const CUtensorMap *map, const void *src, int x, int y, int z) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%1, %2, %3}], [%4];"
+                 ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(src)) : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory"); }
+__device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // ---- shared-memory descriptors (version 1) -----------------------------------------------------------------------------
 // K-major, 128-byte swizzle: 8-row groups 1024 bytes apart; a K step of 32 bytes moves the start address
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
@@ -187,17 +217,20 @@ struct Scales {
     const uint8_t *a, *b;
     size_t lda, ldb;
     uint32_t m, n;
+    uint32_t words;            // both: rows on 4-byte boundaries
 };
 
 // ---- the kernel --------------------------------------------------------------------------------------------------------
-// Epi: a type with `Args`, `Epi(const Args &, uint8_t *staging, int warp_row, int lane)`, `begin(m0, n0, split)`,
-// `chunk(uint32_t (&r)[32], col)` for 32 columns of the lane's row, `end()`.  Every lane of a warp makes the same calls.
+// Epi: a type with `Args`, `Epi(const Args &, uint8_t *staging, const CUtensorMap *out, int lane)`, `begin(first row, first
+// column, split, part)`, `chunk(uint32_t (&r)[32], col)` for 32 columns of the lane's row, `end()` after a tile, `finish()`
+// after the last.  Every lane of a warp makes the same calls.
 template <class S, class Epi>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                           const Grid grid, const Scales scales, const typename Epi::Args epi_args, uint32_t *err) {
+                                                           const __grid_constant__ CUtensorMap map_out, const Grid grid, const Scales scales, const typename Epi::Args epi_args, uint32_t *err) {
     extern __shared__ __align__(1024) uint8_t tile_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tile_smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t full_bar[S::STAGES], empty_bar[S::STAGES], tfull_bar[2], tempty_bar[2], drain_bar;
+    __shared__ uint64_t sfull_bar[S::SCALED ? S::SF_SLOTS : 1], sempty_bar[S::SCALED ? S::SF_SLOTS : 1];
     __shared__ uint32_t tmem_base_s;
     constexpr int CG = S::CG;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -205,8 +238,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     const uint32_t group = blockIdx.x / CG, groups = gridDim.x / CG;
 
     if (tid == 0) {
-        // full: the leader's expect + (e4m3) one arrival per CTA whose scale words are written
-        for (int s = 0; s < S::STAGES; ++s) { mbar_init(&full_bar[s], S::SCALED ? 1 + CG : 1); mbar_init(&empty_bar[s], 1); }
+        for (int s = 0; s < S::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        for (int s = 0; s < S::SF_SLOTS; ++s) { mbar_init(&sfull_bar[s], CG); mbar_init(&sempty_bar[s], 1); }   // an arrival per CTA
         for (int s = 0; s < 2; ++s) { mbar_init(&tfull_bar[s], 1); mbar_init(&tempty_bar[s], kEpiWarps * CG); }
         mbar_init(&drain_bar, 1);
         mbar_fence_init();
@@ -227,23 +260,24 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     const uint32_t tmem = tmem_base_s;
 
     if (warp == kEpiWarps) {
-        // ---------------- TMA producer (every CTA loads its own rows; the pair's leader counts the bytes of both) -------
-        if (lane == 0) {
-            uint32_t g = 0;
-            bool ok = true;
-            for (uint32_t t = group; t < grid.total && ok; t += groups) {
-                uint32_t mi, ni, si;
-                locate(grid, t, mi, ni, si);
-                const int m0 = (int)(mi * S::M + rank * 128), n0 = (int)(ni * S::N + rank * S::BR);
-                const uint32_t k0 = (uint32_t)((uint64_t)grid.kblocks * si / grid.splits), k1 = (uint32_t)((uint64_t)grid.kblocks * (si + 1) / grid.splits);
-                for (uint32_t kb = k0; kb < k1; ++kb, ++g) {
-                    const uint32_t s = g % S::STAGES;
-                    ok = wait(&empty_bar[s], ((g / S::STAGES) & 1u) ^ 1u, err, 30u);
-                    if (!ok) break;
-                    uint8_t *st = smem + (size_t)s * S::STAGE_BYTES;
-                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], S::LOAD_BYTES * CG);
-                    const uint32_t bar = CG == 2 ? leader_addr(&full_bar[s]) : smem_u32(&full_bar[s]);
-                    const int k = (int)(kb * S::K);
+        // ---------------- TMA producer (every CTA loads its own rows; the pair's leader counts the bytes of both) -----------
+        // As in the MMA warp, all lanes walk the loop and one elected lane issues: with the loop inside a one-lane branch the
+        // products were issued at 215 cycles each (e4m3, 112 needed) and 170 (f16, 128 needed).
+        uint32_t s = 0, phase = 0, issued = 0;
+        bool ok = true;
+        for (uint32_t t = group; t < grid.total && ok; t += groups) {
+            uint32_t mi, ni, si;
+            locate(grid, t, mi, ni, si);
+            const int m0 = (int)(mi * S::M + rank * 128), n0 = (int)(ni * S::N + rank * S::BR);
+            const uint32_t k0 = si * grid.kper, k1 = min(k0 + grid.kper, grid.kblocks);
+            for (uint32_t kb = k0; kb < k1; ++kb) {
+                ok = wait(&empty_bar[s], phase ^ 1u, err, 30u);
+                if (!ok) break;
+                uint8_t *st = smem + s * S::STAGE_BYTES;
+                const uint32_t bar = CG == 2 ? leader_addr(&full_bar[s]) : smem_u32(&full_bar[s]);
+                const int k = (int)(kb * S::K);
+                if (elect_one()) {
+                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], S::STAGE_BYTES * CG);
                     if (S::AMN) {
                         load_2d<CG>(st, &map_a, m0, k, bar);
                         load_2d<CG>(st + 8192, &map_a, m0 + 64, k, bar);
@@ -253,94 +287,127 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                         for (int j = 0; j < S::BR / 64; ++j) load_2d<CG>(st + S::A_BYTES + j * 8192, &map_b, n0 + j * 64, k, bar);
                     } else load_2d<CG>(st + S::A_BYTES, &map_b, k, n0, bar);
                 }
+                __syncwarp();
+                ++issued;
+                if (++s == S::STAGES) { s = 0; phase ^= 1u; }
             }
-            if (!ok && rank == 0)   // copies still on their way (both CTAs') complete on these barriers
-                for (uint32_t j = g > S::STAGES ? g - S::STAGES : 0; j < g; ++j) wait(&full_bar[j % S::STAGES], (j / S::STAGES) & 1u, nullptr, 0u, 1u << 12);
         }
-        __syncwarp();
+        if (!ok && rank == 0)   // copies still on their way (both CTAs') complete on these barriers
+            for (uint32_t j = issued > S::STAGES ? issued - S::STAGES : 0; j < issued; ++j)
+                wait(&full_bar[j % S::STAGES], (j / S::STAGES) & 1u, nullptr, 0u, 1u << 12);
     } else if (warp == kEpiWarps + 1) {
-        // ---------------- MMA issue (one lane of the leader) ------------------------------------------------------------
-        if (lane == 0 && rank == 0) {
-            uint32_t g = 0, it = 0;
+        // ---------------- MMA issue (the leader; the warp walks the loop together and one elected lane issues) -----------
+        if (rank == 0) {
+            uint32_t s = 0, phase = 0, it = 0, sg = 0, sf = 0;
             bool ok = true;
             for (uint32_t t = group; t < grid.total && ok; t += groups, ++it) {
-                uint32_t mi, ni, si;
-                locate(grid, t, mi, ni, si);
-                const uint32_t k0 = (uint32_t)((uint64_t)grid.kblocks * si / grid.splits), k1 = (uint32_t)((uint64_t)grid.kblocks * (si + 1) / grid.splits);
+                const uint32_t si = grid.kper < grid.kblocks ? t / (grid.tiles_m * grid.tiles_n) : 0u;
+                const uint32_t k0 = si * grid.kper, k1 = min(k0 + grid.kper, grid.kblocks);
                 const uint32_t acc = it & 1u, d = tmem + acc * S::N;
                 ok = wait(&tempty_bar[acc], ((it >> 1) & 1u) ^ 1u, err, 31u);
                 if (!ok) break;
                 fence_after();
-                for (uint32_t kb = k0; kb < k1; ++kb, ++g) {
-                    const uint32_t s = g % S::STAGES;
-                    ok = wait(&full_bar[s], (g / S::STAGES) & 1u, err, 32u);
+                for (uint32_t kb = k0; kb < k1; ++kb) {
+                    ok = wait(&full_bar[s], phase, err, 32u);
                     if (!ok) break;
+                    const uint32_t slot = sg % (S::SCALED ? S::SF_SLOTS : 1);
+                    const bool fresh = S::SCALED && kb % 4 == 0;
+                    if (fresh) {
+                        // the slot's own scale columns: the products that read them last have completed (their commit freed it)
+                        ok = wait_cluster(&sfull_bar[slot], (sg / (S::SCALED ? S::SF_SLOTS : 1)) & 1u, err, 35u);
+                        if (!ok) break;
+                        sf = tmem + 2 * S::N + slot * 12;
+                    }
                     fence_after();
-                    const uint32_t a = smem_u32(smem + (size_t)s * S::STAGE_BYTES), b = a + S::A_BYTES;
-                    const uint32_t sfa = tmem + 2 * S::N + s * S::SF_COLS, sfb = sfa + 4;
-                    if (S::SCALED) {
-                        // the stage's own scale columns: the products that read them last have completed (their commit freed the stage)
-                        copy_scales<CG>(sfa, desc_sf(b + S::B_BYTES));
-                        copy_scales<CG>(sfb, desc_sf(b + S::B_BYTES + 512));
-                        copy_scales<CG>(sfb + 4, desc_sf(b + S::B_BYTES + 1024));
-                    }
+                    const uint32_t a = smem_u32(smem) + s * S::STAGE_BYTES, b = a + S::A_BYTES;
+                    const uint64_t da = S::AMN ? desc_mn(a) : desc_k(a), db = S::BMN ? desc_mn(b) : desc_k(b);
+                    const uint32_t idesc = S::SCALED ? S::IDESC | ((kb & 3u) << 4) | ((kb & 3u) << 29) : S::IDESC;
+                    if (elect_one()) {
+                        if (fresh) {
+                            const uint32_t w = smem_u32(smem) + S::STAGES * S::STAGE_BYTES + slot * S::SF_BYTES;
+                            copy_scales<CG>(sf, desc_sf(w));
+                            copy_scales<CG>(sf + 4, desc_sf(w + 512));
+                            if (S::N > 128) copy_scales<CG>(sf + 8, desc_sf(w + 1024));
+                        }
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t da = S::AMN ? desc_mn(a + kk * 2048) : desc_k(a + kk * 32);
-                        const uint64_t db = S::BMN ? desc_mn(b + kk * 2048) : desc_k(b + kk * 32);
-                        const uint32_t add = (kb != k0 || kk != 0) ? 1u : 0u;
-                        if (S::SCALED) mma_mx8<CG>(d, da, db, S::IDESC, sfa, sfb, add);
-                        else mma_f16<CG>(d, da, db, S::IDESC, add);
+                        for (int kk = 0; kk < 4; ++kk) {             // the address field counts 16 bytes: 32 or 2048 bytes a step
+                            const uint64_t ia = da + kk * (S::AMN ? 128 : 2), ib = db + kk * (S::BMN ? 128 : 2);
+                            const uint32_t add = (kb != k0 || kk != 0) ? 1u : 0u;
+                            if (S::SCALED) mma_mx8<CG>(d, ia, ib, idesc, sf, sf + 4, add);
+                            else mma_f16<CG>(d, ia, ib, idesc, add);
+                        }
+                        commit<CG>(&empty_bar[s]);
+                        if (S::SCALED && (kb % 4 == 3 || kb + 1 == k1)) commit<CG>(&sempty_bar[slot]);
+                        if (kb + 1 == k1) commit<CG>(&tfull_bar[acc]);
                     }
-                    commit<CG>(&empty_bar[s]);
+                    __syncwarp();
+                    if (S::SCALED && (kb % 4 == 3 || kb + 1 == k1)) ++sg;
+                    if (++s == S::STAGES) { s = 0; phase ^= 1u; }
                 }
-                if (ok) commit<CG>(&tfull_bar[acc]);
             }
             if (!ok) {   // instructions in flight finish before the tensor memory is given back
-                commit<CG>(&drain_bar);
+                if (elect_one()) commit<CG>(&drain_bar);
                 wait(&drain_bar, 0u, nullptr, 0u, 1u << 14);
             }
         }
         __syncwarp();
     } else if (warp >= kEpiWarps + 2) {
-        // ---------------- scale writers (e4m3): the two warps take the K blocks in turn -----------------------------------
-        if (S::SCALED) {
-            uint32_t g = 0;
-            bool ok = true;
-            for (uint32_t t = group; t < grid.total && ok; t += groups) {
+        // ---------------- scale writers (e4m3): the two warps take groups of four K blocks in turn ------------------------
+        // A word of the tensor core's scale layout holds four bytes of a row and every product names the one it uses: the words
+        // are the rows' own bytes of four blocks of 128, copied once per 16 products.  The next group's words are on their way
+        // while the current one waits for its slot.
+        if constexpr (S::SCALED) {
+            constexpr int ROWS = 4 + S::N / 32;
+            const uint32_t per_tile = (grid.kblocks + 3) / 4;        // scaled products are never split
+            uint32_t t = group, grp = (uint32_t)(warp & 1), sg = grp;   // this warp's next group; its number over all tiles
+            auto settle = [&]() { while (t < grid.total && grp >= per_tile) { grp -= per_tile; t += groups; } };
+            auto fetch = [&](uint32_t (&w)[ROWS]) {
                 uint32_t mi, ni, si;
                 locate(grid, t, mi, ni, si);
-                const uint32_t m0 = mi * S::M + rank * 128, n0 = ni * S::N;
-                const uint32_t k0 = (uint32_t)((uint64_t)grid.kblocks * si / grid.splits), k1 = (uint32_t)((uint64_t)grid.kblocks * (si + 1) / grid.splits);
-                for (uint32_t kb = k0; kb < k1 && ok; ++kb, ++g) {
-                    if ((g & 1u) != (uint32_t)(warp & 1)) continue;
-                    const uint32_t s = g % S::STAGES;
-                    // lane i of the 32 lanes keeps rows i, i + 32, i + 64, i + 96 in its 16 bytes; rows past the end: 2^0
-                    uint32_t w[12];
+                const uint32_t m0 = mi * S::M + rank * 128, n0 = ni * S::N, kb = grp * 4;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t row = m0 + j * 32 + lane;
-                        w[j] = row < scales.m ? scales.a[(size_t)row * scales.lda + kb] : 127u;
-                    }
+                for (int j = 0; j < ROWS; ++j) {
+                    const bool of_a = j < 4;
+                    const uint32_t row = of_a ? m0 + j * 32 + lane : n0 + (j - 4) * 32 + lane, rows = of_a ? scales.m : scales.n;
+                    w[j] = 0x7F7F7F7Fu;                              // rows past the end: 2^0
+                    if (row < rows) {
+                        const uint8_t *p = (of_a ? scales.a + (size_t)row * scales.lda : scales.b + (size_t)row * scales.ldb) + kb;
+                        if (scales.words && (kb + 4 <= grid.kblocks || row + 1 < rows)) w[j] = __ldg(reinterpret_cast<const uint32_t *>(p));
+                        else {                                       // all loads independent: none waits for another
+                            uint32_t v[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t row = n0 + j * 32 + lane;
-                        w[4 + j] = j * 32 < S::N && row < scales.n ? scales.b[(size_t)row * scales.ldb + kb] : 127u;
-                    }
-                    ok = wait(&empty_bar[s], ((g / S::STAGES) & 1u) ^ 1u, err, 33u);
-                    ok = __all_sync(0xFFFFFFFFu, ok);
-                    if (!ok) break;
-                    uint4 *dst = reinterpret_cast<uint4 *>(smem + (size_t)s * S::STAGE_BYTES + S::LOAD_BYTES);
-                    dst[lane] = make_uint4(w[0], w[1], w[2], w[3]);
-                    dst[32 + lane] = make_uint4(w[4], w[5], w[6], w[7]);
-                    dst[64 + lane] = make_uint4(w[8], w[9], w[10], w[11]);
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (CG == 2) arrive_cluster(leader_addr(&full_bar[s]));
-                        else mbar_arrive(&full_bar[s]);
+                            for (uint32_t i = 0; i < 4; ++i) v[i] = kb + i < grid.kblocks ? __ldg(p + i) : 127u;
+                            w[j] = v[0] | v[1] << 8 | v[2] << 16 | v[3] << 24;
+                        }
                     }
                 }
+            };
+            uint32_t next[ROWS];
+            settle();
+            if (t < grid.total) fetch(next);
+            bool ok = true;
+            while (t < grid.total) {
+                uint32_t w[12];
+#pragma unroll
+                for (int j = 0; j < 12; ++j) w[j] = j < ROWS ? next[j < ROWS ? j : 0] : 0u;
+                grp += 2;
+                settle();
+                if (t < grid.total) fetch(next);
+                const uint32_t slot = sg % S::SF_SLOTS;
+                ok = __all_sync(0xFFFFFFFFu, wait(&sempty_bar[slot], ((sg / S::SF_SLOTS) & 1u) ^ 1u, err, 33u));
+                if (!ok) break;
+                // lane l of the 32 keeps rows l, l + 32, l + 64, l + 96 in its 16 bytes
+                uint4 *dst = reinterpret_cast<uint4 *>(smem + S::STAGES * S::STAGE_BYTES + slot * S::SF_BYTES);
+                dst[lane] = make_uint4(w[0], w[1], w[2], w[3]);
+                dst[32 + lane] = make_uint4(w[4], w[5], w[6], w[7]);
+                if (S::N > 128) dst[64 + lane] = make_uint4(w[8], w[9], w[10], w[11]);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 2) arrive_cluster_release(leader_addr(&sfull_bar[slot]));
+                    else mbar_arrive(&sfull_bar[slot]);
+                }
+                sg += 2;
             }
         }
     } else {
@@ -348,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         // the columns, 4-7 the second ------------------------------------------------------------------------------------
         const int quarter = warp & 3, half = warp >> 2;
         constexpr int CHUNKS = S::N / 32, FIRST = (CHUNKS + 1) / 2;
-        Epi epi(epi_args, smem + (size_t)S::STAGES * S::STAGE_BYTES + warp * 4096, lane);
+        Epi epi(epi_args, smem + S::STAGES * S::STAGE_BYTES + S::SF_ROOM + warp * 4096, &map_out, lane);
         uint32_t it = 0;
         bool ok = true;
         for (uint32_t t = group; t < grid.total && ok; t += groups, ++it) {
@@ -361,23 +428,36 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             if (!ok) break;
             fence_after();
             const uint32_t src = tmem + ((uint32_t)(32 * quarter) << 16) + acc * S::N;
-            const int c1 = half ? CHUNKS : FIRST;
-            uint32_t r[32];
-            for (int c = half ? FIRST : 0; c < c1; ++c) {
-                tmem_ld32(r, src + c * 32);
-                tmem_wait_ld();
-                if (c == c1 - 1) {          // the last read of this warp: the accumulator can be written again
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (CG == 2) arrive_cluster(leader_addr(&tempty_bar[acc]));
-                        else mbar_arrive(&tempty_bar[acc]);
+            const int c0 = half ? FIRST : 0, c1 = half ? CHUNKS : FIRST;
+            auto release = [&]() {          // the last read of this warp is done: the accumulator can be written again
+                fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 2) arrive_cluster(leader_addr(&tempty_bar[acc]));
+                    else mbar_arrive(&tempty_bar[acc]);
+                }
+            };
+            uint32_t r0[32], r1[32];        // one chunk is worked on while the next one is read
+            tmem_ld32(r0, src + c0 * 32);
+            tmem_wait_ld();
+            if (c1 - c0 == 1) release();
+            for (int c = c0; c < c1; c += 2) {
+                if (c + 1 < c1) tmem_ld32(r1, src + (c + 1) * 32);
+                epi.chunk(r0, ni * S::N + c * 32);
+                if (c + 1 < c1) {
+                    tmem_wait_ld();
+                    if (c + 2 < c1) tmem_ld32(r0, src + (c + 2) * 32);
+                    else release();
+                    epi.chunk(r1, ni * S::N + (c + 1) * 32);
+                    if (c + 2 < c1) {
+                        tmem_wait_ld();
+                        if (c + 3 >= c1) release();
                     }
                 }
-                epi.chunk(r, ni * S::N + c * 32);
             }
             epi.end();
         }
+        epi.finish();
     }
     fence_before();
     __syncthreads();

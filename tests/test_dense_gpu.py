@@ -173,6 +173,25 @@ def test_scores_strides_and_neighbours():
     assert apoe.scaled_scores(qa, sa, qb[:0], sb[:0]).shape == (m, 0)
 
 
+@pytest.mark.parametrize("m", [9, 200])
+@pytest.mark.parametrize("dim", [1, 15, 17, 100, 131, 250])
+def test_scores_ignore_what_lies_behind_a_row(m, dim):
+    g = gen(12)
+    qa, sa = apoe.quantize_rows(torch.randn(m, dim, generator=g, device=DEV))
+    qb, sb = apoe.quantize_rows(torch.randn(70, dim, generator=g, device=DEV))
+    def wide(q, s):                                   # the same rows in the middle of a matrix of the largest values and of NaN
+        room = torch.full((q.shape[0], 272), 0x7E, dtype=torch.uint8, device=DEV)
+        room[1::2] = 0x7F
+        room[:, :dim] = q.view(torch.uint8)
+        scales = torch.full((q.shape[0], 8), 254, dtype=torch.uint8, device=DEV)
+        scales[:, :s.shape[1]] = s
+        return room.view(torch.float8_e4m3fn)[:, :dim], scales[:, :s.shape[1]]
+    (wa, wsa), (wb, wsb) = wide(qa, sa), wide(qb, sb)
+    got = apoe.scaled_scores(wa, wsa, wb, wsb)
+    check_scores(got, qa, sa, qb, sb)
+    assert torch.equal(got, apoe.scaled_scores(qa, sa, qb, sb))
+
+
 # ---- softmax loss ---------------------------------------------------------------------------------------------------------
 def loss_case(rows, docs, dim, dtype, seed, scale=20.0, pad=True):
     g = gen(seed)
@@ -306,6 +325,33 @@ def test_rows_without_a_target_may_hold_anything():
     dq, dd = apoe.softmax_loss_backward(q2, d, t, loss, lse, grad2, scale)
     for a in (loss, lse, dq, dd):
         assert bool((a == 0).all())
+
+
+@pytest.mark.parametrize("rows,docs,dim", [(5, 70, 3), (40, 301, 101), (200, 300, 70), (300, 1029, 131)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_loss_ignores_what_lies_behind_a_row(rows, docs, dim, dtype):
+    """Row lengths that are no multiple of 16 bytes, in rows that are further apart, NaN between them."""
+    q, d, t, scale = loss_case(rows, docs, dim, dtype, 15)
+    wq = torch.full((rows, 136), float("nan"), dtype=dtype, device=DEV)
+    wd = torch.full((docs, 144), float("nan"), dtype=dtype, device=DEV)
+    wq[:, :dim], wd[:, :dim] = q, d
+    vq, vd = wq[:, :dim], wd[:, :dim]
+    grad = torch.full((rows,), (64.0 if dtype == torch.float16 else 1.0) / rows, device=DEV)
+    loss, lse = apoe.softmax_loss_forward(vq, vd, t, scale)
+    want_loss, _ = plain_loss(q, d, t, scale)
+    assert float((loss.double() - want_loss).abs().max()) <= 2 * logit_bound(q, d, scale) + 1e-6
+    dq, dd = apoe.softmax_loss_backward(vq, vd, t, loss, lse, grad, scale)
+    check_grads(q, d, t, scale, grad, loss, lse, dq, dd)
+    # gradients into rows that are further apart: the values between them are left alone (aligned rows, and others)
+    for pad, off in ((152, 0), (137 if dim < 137 else 145, 1)):
+        gq = torch.full((rows, 152), 3.0, dtype=dtype, device=DEV)
+        gd = torch.full((docs * pad + 8,), 3.0, dtype=dtype, device=DEV)[off:off + docs * pad].view(docs, pad)
+        ws, size = apoe._workspace(0, rows, docs, dim, 1)
+        apoe._check(apoe.lib().ap_softmax_loss_backward_device(
+            0, rows, docs, dim, apoe._type_of(dtype), vq.data_ptr(), 136, vd.data_ptr(), 144, t.data_ptr(), scale, loss.data_ptr(), lse.data_ptr(),
+            grad.data_ptr(), gq.data_ptr(), 152, gd.data_ptr(), pad, ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(gq[:, :dim], dq) and torch.equal(gd[:, :dim], dd)
+        assert bool((gq[:, dim:] == 3.0).all()) and bool((gd[:, dim:] == 3.0).all())
 
 
 def test_targets_out_of_range_show_and_give_no_gradient():
