@@ -7,6 +7,7 @@ compute call needs the CUDA library and a device and raises `ApoeError` otherwis
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 import numpy as np
@@ -450,147 +451,161 @@ class Index:
 
 
 # ---- dense operators (CUDA tensors in and out, on the current stream of their device) ---------------------------------
-_TYPES = {}
+_T = None       # torch and what of it the calls below look up each time, set on first use
 
 
-def _type_of(dtype) -> int:
-    if not _TYPES:
+class _Torch:
+    def __init__(self):
         import torch
-        _TYPES.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
-    try:
-        return _TYPES[dtype]
-    except KeyError:
-        raise ApoeError(1, f"{dtype}: float32, float16 and bfloat16 are supported") from None
+        self.torch, self.empty = torch, torch.empty
+        self.f32, self.f16, self.bf16, self.f8, self.u8 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn, torch.uint8
+        self.i32, self.u32 = torch.int32, torch.uint32
+        self.types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+        self.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _matrix(name, t, device=None, dtypes=None):
-    """(device index, rows, columns, row stride) of a CUDA matrix whose rows are contiguous."""
+def _torch():
+    global _T
+    if _T is None:
+        _T = _Torch()
+    return _T
+
+
+def _bad(name, t, device, dtypes):
     if t.dim() != 2 or not t.is_cuda:
         raise ApoeError(1, f"{name}: a CUDA matrix is needed, got {tuple(t.shape)} on {t.device}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ApoeError(1, f"{name}: the values of a row must be contiguous")
-    if device is not None and t.device.index != device:
+    if device >= 0 and t.get_device() != device:
         raise ApoeError(1, f"{name}: is on {t.device}, the other tensors on cuda:{device}")
-    if dtypes is not None and t.dtype not in dtypes:
+    if t.dtype not in dtypes:
         raise ApoeError(1, f"{name}: {t.dtype} where {' or '.join(map(str, dtypes))} is needed")
+    raise ApoeError(1, f"{name}: the values of a row must be contiguous and rows must not overlap (strides {tuple(t.stride())})")
+
+
+def _matrix(name, t, device, dtypes):
+    """(rows, columns, row stride) of a CUDA matrix whose rows are contiguous; device < 0: any."""
+    stride = t.stride()
+    if len(stride) != 2 or not t.is_cuda or (device >= 0 and t.get_device() != device) or t.dtype not in dtypes:
+        _bad(name, t, device, dtypes)
     rows, cols = t.shape
-    ld = t.stride(0) if rows > 1 else max(t.stride(0), cols)
+    ld, step = stride
+    if step != 1 and cols > 1:
+        _bad(name, t, device, dtypes)
     if ld < cols:
-        raise ApoeError(1, f"{name}: rows overlap (stride {ld}, {cols} values)")
-    return t.device.index, rows, cols, ld
+        if rows > 1:
+            _bad(name, t, device, dtypes)
+        ld = cols
+    return rows, cols, ld
 
 
 def _vector(name, t, n, device, dtypes):
-    if t.dim() != 1 or t.shape[0] != n or not t.is_cuda or t.device.index != device or not t.is_contiguous() or t.dtype not in dtypes:
+    if t.dtype not in dtypes or t.dim() != 1 or t.numel() != n or t.get_device() != device or not t.is_contiguous():
         raise ApoeError(1, f"{name}: a contiguous vector of {n} {' or '.join(map(str, dtypes))} on cuda:{device} is needed, "
                            f"got {tuple(t.shape)} {t.dtype} on {t.device}")
-
-
-def _stream(device, stream):
-    if stream is not None:
-        return stream
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    return t.data_ptr()
 
 
 def quantize_rows(x, stream=None):
     """Rows in 8 bits: (q float8_e4m3fn [rows, dim], scale uint8 [rows, ceil(dim / 128)]).  The value of q[r, c] is
     q * 2^(scale[r, c // 128] - 127).  x: float32, float16 or bfloat16 matrix.  The rows of q start on 16-byte boundaries."""
-    import torch
-    kind = _type_of(x.dtype)
-    device, rows, dim, ld = _matrix("x", x)
+    T = _T or _torch()
+    rows, dim, ld = _matrix("x", x, -1, T.types)
     if dim == 0:
         raise ApoeError(1, "quantize: rows of 0 values")
+    device = x.get_device()
     ldq, blocks = (dim + 15) // 16 * 16, (dim + 127) // 128
-    q = torch.empty(rows, ldq, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(rows, blocks, dtype=torch.uint8, device=x.device)
-    _check(lib().ap_quantize_rows_device(device, rows, dim, kind, x.data_ptr(), ld, q.data_ptr(), ldq, scale.data_ptr(), blocks,
-                                         _stream(device, stream)))
+    q = x.new_empty((rows, ldq), dtype=T.f8)
+    scale = x.new_empty((rows, blocks), dtype=T.u8)
+    _check(lib().ap_quantize_rows_device(device, rows, dim, T.types[x.dtype], x.data_ptr(), ld, q.data_ptr(), ldq, scale.data_ptr(), blocks,
+                                         T.stream(device) if stream is None else stream))
     return (q if ldq == dim else q[:, :dim]), scale
 
 
 def scaled_scores(a, a_scale, b, b_scale, out_dtype=None, alpha: float = 1.0, out=None, stream=None):
     """Scores of 8-bit rows (as `quantize_rows` returns them): [rows of a, rows of b] in out_dtype (float32 by default,
     float16, bfloat16), summed in fp32.  Rows of a and b must start on 16-byte boundaries."""
-    import torch
-    f8, u8 = (torch.float8_e4m3fn,), (torch.uint8,)
-    device, m, dim, lda = _matrix("a", a, None, f8)
-    _, n, dim_b, ldb = _matrix("b", b, device, f8)
+    T = _T or _torch()
+    m, dim, lda = _matrix("a", a, -1, (T.f8,))
+    device = a.get_device()
+    n, dim_b, ldb = _matrix("b", b, device, (T.f8,))
     if dim != dim_b:
         raise ApoeError(1, f"scores: rows of {dim} and of {dim_b} values")
     blocks = (dim + 127) // 128
-    _, ma, ca, lsa = _matrix("a_scale", a_scale, device, u8)
-    _, nb, cb, lsb = _matrix("b_scale", b_scale, device, u8)
-    if (ma, ca, nb, cb) != (m, blocks, n, blocks):
+    ma, ca, lsa = _matrix("a_scale", a_scale, device, (T.u8,))
+    nb, cb, lsb = _matrix("b_scale", b_scale, device, (T.u8,))
+    if ma != m or nb != n or ca != blocks or cb != blocks:
         raise ApoeError(1, f"scores: scales {ma} x {ca} and {nb} x {cb}, needed {m} x {blocks} and {n} x {blocks}")
     if out is None:
-        out = torch.empty(m, n, dtype=out_dtype or torch.float32, device=a.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        raise ApoeError(1, f"scores: out is {out.dtype}, out_dtype {out_dtype}")
-    kind = _type_of(out.dtype)
-    _, om, on, ldo = _matrix("out", out, device)
-    if (om, on) != (m, n):
-        raise ApoeError(1, f"scores: out is {om} x {on}, needed {m} x {n}")
-    ra = ScaledRows(m, a.data_ptr(), lda, a_scale.data_ptr(), lsa)
-    rb = ScaledRows(n, b.data_ptr(), ldb, b_scale.data_ptr(), lsb)
-    _check(lib().ap_scaled_scores_device(device, dim, ra, rb, alpha, kind, out.data_ptr(), ldo, _stream(device, stream)))
+        out = a.new_empty((m, n), dtype=out_dtype or T.f32)
+        ldo = n
+    else:
+        om, on, ldo = _matrix("out", out, device, T.types)
+        if om != m or on != n:
+            raise ApoeError(1, f"scores: out is {om} x {on}, needed {m} x {n}")
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ApoeError(1, f"scores: out is {out.dtype}, out_dtype {out_dtype}")
+    kind = T.types.get(out.dtype)
+    if kind is None:
+        raise ApoeError(1, f"scores: {out.dtype}: float32, float16 and bfloat16 are supported")
+    _check(lib().ap_scaled_scores_device(device, dim, ScaledRows(m, a.data_ptr(), lda, a_scale.data_ptr(), lsa),
+                                         ScaledRows(n, b.data_ptr(), ldb, b_scale.data_ptr(), lsb), alpha, kind, out.data_ptr(), ldo,
+                                         T.stream(device) if stream is None else stream))
     return out
 
 
-def _loss_args(queries, docs, target):
-    import torch
-    half = (torch.float16, torch.bfloat16)
-    device, rows, dim, ldq = _matrix("queries", queries, None, half)
-    _, n, dim_d, ldd = _matrix("docs", docs, device, (queries.dtype,))
+def _loss_args(T, queries, docs, target):
+    rows, dim, ldq = _matrix("queries", queries, -1, (T.f16, T.bf16))
+    device = queries.get_device()
+    n, dim_d, ldd = _matrix("docs", docs, device, (queries.dtype,))
     if dim != dim_d:
         raise ApoeError(1, f"softmax loss: queries of {dim} values, documents of {dim_d}")
-    _vector("target", target, rows, device, (torch.int32, torch.uint32))
-    return device, rows, n, dim, _type_of(queries.dtype), ldq, ldd
+    return device, rows, n, dim, T.types[queries.dtype], queries.data_ptr(), ldq, docs.data_ptr(), ldd, \
+        _vector("target", target, rows, device, (T.i32, T.u32))
 
 
-def _workspace(device, rows, n, dim, backward):
-    import torch
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(device, rows, n, dim, backward):
     size = C.c_size_t(0)
     _check(lib().ap_softmax_loss_workspace(device, rows, n, dim, backward, size))
-    return torch.empty(size.value, dtype=torch.uint8, device=torch.device("cuda", device)), size.value
+    return size.value
 
 
 def softmax_loss_forward(queries, docs, target, scale: float = 1.0, stream=None):
     """Softmax loss of queries over all documents without holding the matrix of scores: (loss, lse), float32 [rows].
     queries [rows, dim] and docs [n, dim]: float16 or bfloat16; target: int32 document ids, -1 = the row takes no part."""
-    import torch
-    device, rows, n, dim, kind, ldq, ldd = _loss_args(queries, docs, target)
-    out = torch.empty(2, rows, dtype=torch.float32, device=queries.device)
-    loss, lse = out[0], out[1]
-    ws, size = _workspace(device, rows, n, dim, 0)
-    _check(lib().ap_softmax_loss_forward_device(device, rows, n, dim, kind, queries.data_ptr(), ldq, docs.data_ptr(), ldd, target.data_ptr(),
-                                                scale, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size, _stream(device, stream)))
+    T = _T or _torch()
+    args = _loss_args(T, queries, docs, target)
+    device, rows, n, dim = args[:4]
+    size = _workspace_bytes(device, rows, n, dim, 0)
+    ws = queries.new_empty(size, dtype=T.u8)
+    loss, lse = queries.new_empty(rows, dtype=T.f32), queries.new_empty(rows, dtype=T.f32)
+    _check(lib().ap_softmax_loss_forward_device(*args, scale, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size,
+                                                T.stream(device) if stream is None else stream))
     return loss, lse
 
 
 def softmax_loss_backward(queries, docs, target, loss, lse, grad_loss, scale: float = 1.0, stream=None):
     """Gradients of `softmax_loss_forward`: (grad_queries, grad_docs) in the vectors' type.  loss, lse: as the forward call
     returned them; grad_loss: float32 [rows], the gradient of each row's loss (1 / rows for a mean)."""
-    import torch
-    device, rows, n, dim, kind, ldq, ldd = _loss_args(queries, docs, target)
-    f32 = (torch.float32,)
-    _vector("loss", loss, rows, device, f32)
-    _vector("lse", lse, rows, device, f32)
-    _vector("grad_loss", grad_loss, rows, device, f32)
+    T = _T or _torch()
+    args = _loss_args(T, queries, docs, target)
+    device, rows, n, dim = args[:4]
+    f32 = (T.f32,)
+    pl, pe = _vector("loss", loss, rows, device, f32), _vector("lse", lse, rows, device, f32)
+    pg = _vector("grad_loss", grad_loss, rows, device, f32)
     pad = (dim + 7) // 8 * 8
-    gq = torch.empty(rows, pad, dtype=queries.dtype, device=queries.device)
-    gd = torch.empty(n, pad, dtype=queries.dtype, device=queries.device)
-    ws, size = _workspace(device, rows, n, dim, 1)
-    _check(lib().ap_softmax_loss_backward_device(device, rows, n, dim, kind, queries.data_ptr(), ldq, docs.data_ptr(), ldd, target.data_ptr(),
-                                                 scale, loss.data_ptr(), lse.data_ptr(), grad_loss.data_ptr(), gq.data_ptr(), pad,
-                                                 gd.data_ptr(), pad, ws.data_ptr(), size, _stream(device, stream)))
+    gq, gd = queries.new_empty((rows, pad)), queries.new_empty((n, pad))
+    size = _workspace_bytes(device, rows, n, dim, 1)
+    ws = queries.new_empty(size, dtype=T.u8)
+    _check(lib().ap_softmax_loss_backward_device(*args, scale, pl, pe, pg, gq.data_ptr(), pad, gd.data_ptr(), pad, ws.data_ptr(), size,
+                                                 T.stream(device) if stream is None else stream))
     return (gq, gd) if pad == dim else (gq[:, :dim], gd[:, :dim])
 
 
 def dense_check_status(device: int = 0, stream=None) -> None:
     """Waits for the stream (the device's current one by default) and raises ApoeError(6) when a bounded wait of an earlier
     dense operator ran out."""
-    _check(lib().ap_dense_check_status(device, _stream(device, stream)))
+    T = _T or _torch()
+    _check(lib().ap_dense_check_status(device, T.stream(device) if stream is None else stream))
 
 
 def build_index(dense_path, sparse_path, bm25_path, out_path, device=0, iterations=0, seed=0, flags=0) -> BuildStats:

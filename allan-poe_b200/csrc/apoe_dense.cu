@@ -10,6 +10,7 @@
 // ever held whole: the loss keeps a running maximum and sum per row and column tile, the gradients recompute the logits of
 // one piece of the documents at a time.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <mutex>
 
@@ -79,66 +80,83 @@ struct QuantArgs {
     const void *src;
     uint8_t *q, *scale;
     size_t lds, ldq, ldsc;     // row strides: elements of src, bytes of q and scale
-    uint64_t items;            // rows x blocks
+    uint32_t items;            // rows x blocks
     uint32_t dim, blocks;
-    uint32_t vec;              // src and q rows allow 16-byte (f32) / 8-byte (f16, bf16) accesses
+    uint32_t vec;              // src and q rows allow 16-byte loads and the stores that go with them
 };
 
-// One warp per block of 128 values, kQuantUnroll neighbouring blocks in flight: memory-bound, one pass.  Each lane holds four
-// consecutive values of a block (16 bytes of f32, 8 bytes of f16 / bf16), five shuffles give the block's maximum.
+// One pass, bound by memory.  A lane holds 16 bytes of a block: the 32 lanes of a warp one block of f32, two blocks of f16 or
+// bf16; shuffles give each block's maximum.  A warp has four such loads in flight, of neighbouring blocks.
 constexpr int kQuantUnroll = 4;
 template <class T>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantArgs a) {
-    const int lane = threadIdx.x & 31;
-    const uint64_t w0 = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    for (uint64_t first = w0 * kQuantUnroll; first < a.items; first += (uint64_t)gridDim.x * (blockDim.x >> 5) * kQuantUnroll) {
-        float v[kQuantUnroll][4];
-        uint64_t row[kQuantUnroll];
-        uint32_t blk[kQuantUnroll];
+    constexpr int V = 16 / (int)sizeof(T), LANES = 128 / V, PER = 32 / LANES;   // values of a lane, lanes and blocks of a load
+    constexpr uint32_t STEP = kQuantUnroll * PER;
+    const uint32_t lane = threadIdx.x & 31, sub = lane / LANES, c0 = (lane % LANES) * V;
+    const uint32_t warps = gridDim.x * (blockDim.x >> 5), warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    tile::pdl_launch();
+    tile::pdl_wait();
+    const uint32_t rounds = (a.items - 1) / STEP + 1;
+    for (uint32_t round = warp; round < rounds; round += warps) {
+        uint32_t row[kQuantUnroll], blk[kQuantUnroll];
+        bool live[kQuantUnroll];
+        uint4 raw[kQuantUnroll];
+        const uint32_t it0 = round * STEP + sub;
+        uint32_t r = it0 / a.blocks, b = it0 - r * a.blocks;
 #pragma unroll
         for (int u = 0; u < kQuantUnroll; ++u) {
-            const uint64_t it = first + u;
-            row[u] = it / a.blocks;
-            blk[u] = (uint32_t)(it - row[u] * a.blocks);
-            const uint32_t c = blk[u] * 128 + lane * 4;
+            live[u] = it0 + u * PER < a.items && it0 + u * PER >= it0;
+            row[u] = r; blk[u] = b;
+            b += PER;
+            while (b >= a.blocks) { b -= a.blocks; ++r; }
+            raw[u] = make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t c = blk[u] * 128 + c0;
+            if (live[u] && c < a.dim) {
+                const T *p = static_cast<const T *>(a.src) + (size_t)row[u] * a.lds + c;
+                if (a.vec && c + V <= a.dim) raw[u] = __ldcs(reinterpret_cast<const uint4 *>(p));
+                else {
+                    uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[u][i] = 0.0f;
-            if (it < a.items) {
-                const T *p = static_cast<const T *>(a.src) + row[u] * a.lds + c;
-                if (a.vec && c + 4 <= a.dim) {
-                    if constexpr (sizeof(T) == 4) {
-                        const float4 f = __ldcs(reinterpret_cast<const float4 *>(p));
-                        v[u][0] = f.x; v[u][1] = f.y; v[u][2] = f.z; v[u][3] = f.w;
-                    } else {
-                        const uint2 h = __ldcs(reinterpret_cast<const uint2 *>(p));
-                        const float2 lo = Half16<T>::unpack(h.x), hi = Half16<T>::unpack(h.y);
-                        v[u][0] = lo.x; v[u][1] = lo.y; v[u][2] = hi.x; v[u][3] = hi.y;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) if (c + i < a.dim) v[u][i] = load_as_float(p + i);
+                    for (int i = 0; i < V; ++i)
+                        if (c + i < a.dim) {
+                            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
+                            else w[i / 2] |= (uint32_t)*reinterpret_cast<const uint16_t *>(p + i) << (16 * (i & 1));
+                        }
+                    raw[u] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
 #pragma unroll
         for (int u = 0; u < kQuantUnroll; ++u) {
+            float v[V];
+            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+                else { const float2 f = Half16<T>::unpack(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+            }
             float m = 0.0f;                                  // a NaN is never taken: fmaxf returns the other one
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(v[u][i]));
+            for (int i = 0; i < V; ++i) m = fmaxf(m, fabsf(v[i]));
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+            for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
             const int e = block_exponent(m);
             const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-            if (first + u >= a.items) continue;
-            const uint32_t c = blk[u] * 128 + lane * 4;
-            const uint32_t p = e4m3x2(v[u][0] * down, v[u][1] * down) | (e4m3x2(v[u][2] * down, v[u][3] * down) << 16);
-            uint8_t *o = a.q + row[u] * a.ldq + c;
-            if (a.vec && c + 4 <= a.dim) *reinterpret_cast<uint32_t *>(o) = p;
-            else {
+            const uint32_t c = blk[u] * 128 + c0;
+            if (!live[u] || c >= a.dim) continue;
+            uint32_t p[V / 4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) if (c + i < a.dim) o[i] = (uint8_t)(p >> (8 * i));
+            for (int i = 0; i < V / 4; ++i)
+                p[i] = e4m3x2(v[4 * i] * down, v[4 * i + 1] * down) | (e4m3x2(v[4 * i + 2] * down, v[4 * i + 3] * down) << 16);
+            uint8_t *o = a.q + (size_t)row[u] * a.ldq + c;
+            if (a.vec && c + V <= a.dim) {
+                if constexpr (V == 4) *reinterpret_cast<uint32_t *>(o) = p[0];
+                else *reinterpret_cast<uint2 *>(o) = make_uint2(p[0], p[1]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) if (c + i < a.dim) o[i] = (uint8_t)(p[i / 4] >> (8 * (i & 3)));
             }
-            if (lane == 0) a.scale[row[u] * a.ldsc + blk[u]] = (uint8_t)(e + 127);
+            if (c0 == 0) a.scale[(size_t)row[u] * a.ldsc + blk[u]] = (uint8_t)(e + 127);
         }
     }
 }
@@ -336,6 +354,8 @@ struct JoinArgs {
 // row is nearly certain (z << 0) and where it is hopeless; lse = target's logit + loss.
 template <class T>
 __global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs a) {
+    tile::pdl_launch();
+    tile::pdl_wait();
     const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= a.rows) return;
     float top = -1.0e30f, sum = 0.f;
@@ -401,6 +421,8 @@ struct PrepArgs {
 // inside a product); block 0 also finds the factor of G from the largest |grad| of the rows that count.
 template <class T>
 __global__ void __launch_bounds__(256) grad_prep_kernel(const PrepArgs a) {
+    tile::pdl_launch();
+    tile::pdl_wait();
     if (blockIdx.x == 0) {
         __shared__ float s[8];
         float m = 0.f;
@@ -441,6 +463,8 @@ struct FinishArgs {
 // dX from the partial sums of the splits (added in a fixed order), rounded once
 template <class T>
 __global__ void __launch_bounds__(256) grad_finish_kernel(const FinishArgs a) {
+    tile::pdl_launch();
+    tile::pdl_wait();
     const float f = a.factor[1];
     const uint32_t quads = (a.dim + 3) / 4;
     const uint64_t total = (uint64_t)a.rows * quads;
@@ -512,6 +536,22 @@ struct Operand {   // a stored matrix: rows x cols, row stride in values
 };
 static uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
+// A kernel of 256 threads, started while the one before it ends (every kernel here waits for that before it reads or writes)
+template <class Args>
+static int launch(void (*kernel)(Args), uint32_t grid, const Args &args, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    AP_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
+    return AP_OK;
+}
+
 // C[m][n] = sum over k of A B^T on one shape, K cut into at most `splits` parts.  K-major operands are stored rows x K, MN-major ones K x rows.
 template <class S, class Epi>
 static int tile_launch(const Operand &a, const Operand &b, uint32_t m, uint32_t n, uint32_t k, uint32_t splits, const Scales &sc,
@@ -529,26 +569,45 @@ static int tile_launch(const Operand &a, const Operand &b, uint32_t m, uint32_t 
     // row tiles that walk the columns together: all of them while their operand stays in L2 (32 MB of it), else 8
     const uint64_t row_bytes = (uint64_t)S::M * k * (S::SCALED ? 1 : 2);
     g.group_m = std::min<uint32_t>(g.tiles_m, (uint32_t)std::max<uint64_t>(8, (32ull << 20) / row_bytes));
-    AP_CUDA(cudaFuncSetAttribute(tile::tile_kernel<S, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
+    static std::atomic<uint64_t> allowed{0};    // devices on which this kernel's shared-memory size has been set
+    int device = 0;
+    AP_CUDA(cudaGetDevice(&device));
+    if (device >= 64 || !(allowed.load(std::memory_order_acquire) >> device & 1)) {
+        AP_CUDA(cudaFuncSetAttribute(tile::tile_kernel<S, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
+        if (device < 64) allowed.fetch_or(1ull << device, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(std::min<uint32_t>(g.total, (uint32_t)sms / S::CG) * S::CG);
     cfg.blockDim = dim3(tile::kThreads);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = S::CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = S::CG; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     AP_CUDA(cudaLaunchKernelEx(&cfg, tile::tile_kernel<S, Epi>, ma, mb, mo, g, sc, epi, err));
     return AP_OK;
 }
 
+// SM count and address of the error word, looked up once per device
 static int device_facts(int device, int *sms, uint32_t **err) {
-    AP_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
-    void *p = nullptr;
-    AP_CUDA(cudaGetSymbolAddress(&p, dense_error_word));
-    *err = static_cast<uint32_t *>(p);
+    struct Facts { std::atomic<uint32_t *> err{nullptr}; int sms = 0; };
+    static Facts facts[64];
+    static std::mutex mu;
+    if (device < 0 || device >= 64) return fail(AP_ERR_ARG, "device %d", device);
+    Facts &f = facts[device];
+    if (!f.err.load(std::memory_order_acquire)) {
+        std::lock_guard<std::mutex> lock(mu);
+        AP_CUDA(cudaDeviceGetAttribute(&f.sms, cudaDevAttrMultiProcessorCount, device));
+        void *p = nullptr;
+        AP_CUDA(cudaGetSymbolAddress(&p, dense_error_word));
+        f.err.store(static_cast<uint32_t *>(p), std::memory_order_release);
+    }
+    *sms = f.sms;
+    *err = f.err.load(std::memory_order_acquire);
     return AP_OK;
 }
 static bool aligned(const void *p, uint64_t stride_bytes, uint64_t to) { return (uintptr_t)p % to == 0 && stride_bytes % to == 0; }
@@ -617,8 +676,7 @@ static int forward_run(const LossCall &c, const ForwardPlan &p, uint8_t *ws, flo
         AP_TRY((tile_launch<S, LseEpi>(x, w, c.rows, n, c.dim, 1, Scales{}, ea, c.sms, c.err, c.st)));
         JoinArgs ja{part, carry, c.x, c.w, c.ldx, c.ldw, c.target, loss, lse, c.rows, c.docs, c.dim, ea.parts, v0 == 0 ? 1u : 0u,
                     v0 + n == c.docs ? 1u : 0u, c.scale};
-        loss_join_kernel<T><<<ceil_div(c.rows, 8), 256, 0, c.st>>>(ja);
-        AP_CUDA(cudaGetLastError());
+        AP_TRY(launch(loss_join_kernel<T>, ceil_div(c.rows, 8), ja, c.st));
     }
     return AP_OK;
 }
@@ -634,8 +692,7 @@ static int backward_run(const LossCall &c, const BackwardPlan &p, uint8_t *ws, c
     T *xc = reinterpret_cast<T *>(ws + p.x_off), *g = reinterpret_cast<T *>(ws + p.g_off);
     float *part = reinterpret_cast<float *>(ws + p.p_off);
     PrepArgs pa{c.x, xc, c.ldx, p.ldx, c.target, grad, factor, c.rows, c.docs, c.dim, c.scale};
-    grad_prep_kernel<T><<<1 + std::min<uint32_t>(ceil_div(c.rows, 8), 4 * (uint32_t)c.sms), 256, 0, c.st>>>(pa);
-    AP_CUDA(cudaGetLastError());
+    AP_TRY(launch(grad_prep_kernel<T>, 1 + std::min<uint32_t>(ceil_div(c.rows, 8), 4 * (uint32_t)c.sms), pa, c.st));
     const Operand x{xc, c.rows, c.dim, p.ldx};
     for (uint32_t v0 = 0; v0 < c.docs; v0 += p.piece) {
         const uint32_t n = std::min(p.piece, c.docs - v0);
@@ -657,9 +714,7 @@ static int backward_run(const LossCall &c, const BackwardPlan &p, uint8_t *ws, c
     }
     FinishArgs fa{part, factor, dx, p.ldp, lddx, c.rows, c.dim, p.splits};
     const uint64_t quads = (uint64_t)c.rows * ((c.dim + 3) / 4);
-    grad_finish_kernel<T><<<(uint32_t)std::min<uint64_t>((quads + 255) / 256, 8ull * c.sms), 256, 0, c.st>>>(fa);
-    AP_CUDA(cudaGetLastError());
-    return AP_OK;
+    return launch(grad_finish_kernel<T>, (uint32_t)std::min<uint64_t>((quads + 255) / 256, 8ull * c.sms), fa, c.st);
 }
 
 // ---- scores: the shapes ---------------------------------------------------------------------------------------------------
@@ -724,20 +779,21 @@ extern "C" int ap_quantize_rows_device(int device, uint32_t rows, uint32_t dim, 
     if (!src || !q || !scale) return fail(AP_ERR_ARG, "quantize: null argument");
     const uint32_t blocks = ceil_div(dim, 128);
     if (ld < dim || ldq < dim || ld_scale < blocks) return fail(AP_ERR_ARG, "quantize: a row stride is shorter than a row");
+    if ((uint64_t)rows * blocks >= (1ull << 32)) return fail(AP_ERR_LIMIT, "quantize: %u rows of %u blocks in one call", rows, blocks);
     if ((uintptr_t)src % (uint32_t)size) return fail(AP_ERR_ARG, "quantize: the source is not aligned to its type");
     DeviceScope scope;
     AP_TRY(scope.enter(device));
     int sms;
-    AP_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-    QuantArgs a{src, q, scale, ld, ldq, ld_scale, (uint64_t)rows * blocks, dim, blocks, 0};
-    a.vec = aligned(src, ld * size, 4 * size) && aligned(q, ldq, 4);
-    const uint32_t grid = (uint32_t)std::min<uint64_t>((a.items + 8 * kQuantUnroll - 1) / (8 * kQuantUnroll), 8ull * sms);
+    uint32_t *err;
+    AP_TRY(device_facts(device, &sms, &err));
+    QuantArgs a{src, q, scale, ld, ldq, ld_scale, rows * blocks, dim, blocks, 0};
+    a.vec = aligned(src, ld * size, 16) && aligned(q, ldq, 16 / size);
+    const uint32_t step = kQuantUnroll * 8 * (size == 4 ? 1 : 2);
+    const uint32_t grid = std::min<uint32_t>((a.items - 1) / step + 1, 8 * (uint32_t)sms);
     cudaStream_t st = (cudaStream_t)stream;
-    if (type == AP_TYPE_F32) quantize_kernel<float><<<grid, 256, 0, st>>>(a);
-    else if (type == AP_TYPE_F16) quantize_kernel<__half><<<grid, 256, 0, st>>>(a);
-    else quantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-    AP_CUDA(cudaGetLastError());
-    return AP_OK;
+    if (type == AP_TYPE_F32) return launch(quantize_kernel<float>, grid, a, st);
+    if (type == AP_TYPE_F16) return launch(quantize_kernel<__half>, grid, a, st);
+    return launch(quantize_kernel<__nv_bfloat16>, grid, a, st);
 }
 
 extern "C" int ap_scaled_scores_device(int device, uint32_t dim, const ap_scaled_rows *a, const ap_scaled_rows *b, float alpha, uint32_t out_type, void *out,

@@ -81,6 +81,12 @@ __device__ __forceinline__ void locate(const Grid &g, uint32_t id, uint32_t &mi,
     mi = grp * g.group_m + (r - ni * rows);
 }
 
+// Programmatic launch: the next kernel of the stream may start (as far as SMs are free) / wait until the kernels before this
+// one have ended and their writes are visible.  Every kernel of the dense operators does both, the wait before any access to
+// global memory, so kernels end in order.
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- instructions ----------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -237,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
     const uint32_t group = blockIdx.x / CG, groups = gridDim.x / CG;
 
+    pdl_launch();
     if (tid == 0) {
         for (int s = 0; s < S::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
         for (int s = 0; s < S::SF_SLOTS; ++s) { mbar_init(&sfull_bar[s], CG); mbar_init(&sempty_bar[s], 1); }   // an arrival per CTA
@@ -258,6 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     if (CG == 2) cluster_sync();
     fence_after();
     const uint32_t tmem = tmem_base_s;
+    pdl_wait();
 
     if (warp == kEpiWarps) {
         // ---------------- TMA producer (every CTA loads its own rows; the pair's leader counts the bytes of both) -----------

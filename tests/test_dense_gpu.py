@@ -346,9 +346,10 @@ def test_loss_ignores_what_lies_behind_a_row(rows, docs, dim, dtype):
     for pad, off in ((152, 0), (137 if dim < 137 else 145, 1)):
         gq = torch.full((rows, 152), 3.0, dtype=dtype, device=DEV)
         gd = torch.full((docs * pad + 8,), 3.0, dtype=dtype, device=DEV)[off:off + docs * pad].view(docs, pad)
-        ws, size = apoe._workspace(0, rows, docs, dim, 1)
+        size = apoe._workspace_bytes(0, rows, docs, dim, 1)
+        ws = torch.empty(size, dtype=torch.uint8, device=DEV)
         apoe._check(apoe.lib().ap_softmax_loss_backward_device(
-            0, rows, docs, dim, apoe._type_of(dtype), vq.data_ptr(), 136, vd.data_ptr(), 144, t.data_ptr(), scale, loss.data_ptr(), lse.data_ptr(),
+            0, rows, docs, dim, {torch.float16: 1, torch.bfloat16: 2}[dtype], vq.data_ptr(), 136, vd.data_ptr(), 144, t.data_ptr(), scale, loss.data_ptr(), lse.data_ptr(),
             grad.data_ptr(), gq.data_ptr(), 152, gd.data_ptr(), pad, ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream))
         assert torch.equal(gq[:, :dim], dq) and torch.equal(gd[:, :dim], dd)
         assert bool((gq[:, dim:] == 3.0).all()) and bool((gd[:, dim:] == 3.0).all())
