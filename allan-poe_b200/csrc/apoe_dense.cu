@@ -183,12 +183,12 @@ struct StoreEpi {
     static constexpr int UNITS = (int)sizeof(T) / 2;       // boxes of 32 columns
     static constexpr int COLS = 32 / UNITS;                // columns of a box
     const Args &a;
-    uint8_t *st;
+    tile::Staging &st;
     const CUtensorMap *map;
     int lane;
     float alpha;
-    uint32_t row0 = 0, split = 0, boxes = 0;
-    __device__ __forceinline__ StoreEpi(const Args &args, uint8_t *staging, const CUtensorMap *out, int lane_) : a(args), st(staging), map(out), lane(lane_) {
+    uint32_t row0 = 0, split = 0;
+    __device__ __forceinline__ StoreEpi(const Args &args, tile::Staging &staging, const CUtensorMap *out, int lane_) : a(args), st(staging), map(out), lane(lane_) {
         alpha = a.alpha_dev ? a.alpha * __ldg(a.alpha_dev) : a.alpha;
     }
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t s, uint32_t) { row0 = r0; split = s; }
@@ -205,12 +205,12 @@ struct StoreEpi {
         for (int u = 0; u < UNITS; ++u) {
             const uint32_t c = col + u * COLS;
             if (c >= a.n) return;
-            uint8_t *box = st + (boxes & 1) * 2048;
-            if (boxes >= 2) {                              // the box written two rounds ago has left
+            uint8_t *box = st.base + (st.boxes & 1) * 2048;
+            if (st.boxes >= 2) {                              // the box written two rounds ago has left
                 if (lane == 0) tile::store_wait_read<1>();
                 __syncwarp();
             }
-            ++boxes;
+            ++st.boxes;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t p[4];
@@ -263,7 +263,7 @@ struct LseEpi {
     int lane;
     uint32_t row = 0, part = 0, tgt = 0;
     float top = 0.f, sum = 0.f;
-    __device__ __forceinline__ LseEpi(const Args &args, uint8_t *, const CUtensorMap *, int lane_) : a(args), lane(lane_) {}
+    __device__ __forceinline__ LseEpi(const Args &args, tile::Staging &, const CUtensorMap *, int lane_) : a(args), lane(lane_) {}
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t, uint32_t p) {
         row = r0 + lane; part = p;
         tgt = row < a.m ? __ldg(a.target + row) - a.col0 : kNoTarget;   // columns are below 2^31: no match for a target of another piece
@@ -309,7 +309,7 @@ struct GradEpi {
     StoreEpi<T> store;
     uint32_t tgt = 0;
     float lse2 = 0.f, g = 0.f, at_target = 0.f;
-    __device__ __forceinline__ GradEpi(const Args &args, uint8_t *staging, const CUtensorMap *out, int lane) : a(args), store(args.out, staging, out, lane) {}
+    __device__ __forceinline__ GradEpi(const Args &args, tile::Staging &staging, const CUtensorMap *out, int lane) : a(args), store(args.out, staging, out, lane) {}
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t n0, uint32_t s, uint32_t p) {
         store.begin(r0, n0, s, p);
         const uint32_t row = r0 + store.lane;
@@ -552,32 +552,63 @@ static int launch(void (*kernel)(Args), uint32_t grid, const Args &args, cudaStr
     return AP_OK;
 }
 
-// C[m][n] = sum over k of A B^T on one shape, K cut into at most `splits` parts.  K-major operands are stored rows x K, MN-major ones K x rows.
-template <class S, class Epi>
-static int tile_launch(const Operand &a, const Operand &b, uint32_t m, uint32_t n, uint32_t k, uint32_t splits, const Scales &sc,
-                       const typename Epi::Args &epi, int sms, uint32_t *err, cudaStream_t st) {
-    CUtensorMap ma, mb, mo = {};
-    AP_TRY(make_map_2d(&ma, S::KIND, a.base, a.rows, a.cols, a.ld, S::AMN ? 64 : 128));
-    AP_TRY(make_map_2d(&mb, S::KIND, b.base, b.rows, b.cols, b.ld, S::BMN ? 64 : S::BR));
-    Grid g;
+// What a tile costs, in K blocks of a full tile (about 0.5 us on a pair of SMs): its K blocks, each in proportion to its columns
+// and its rows' share of the loads but never below 0.6 of a full one, and 1.5 for its ends; a short K leaves the epilogue
+// (2.5 us for 256 columns) to wait for.  Measured on pairs at K = 2048, us per K block: 16 bits 0.34 / 0.41 / 0.51 at 128 / 192 /
+// 256 columns, 8 bits 0.36 / 0.39 / 0.48 / 0.53 at 32 to 96 / 128 / 192 / 224.
+static double tile_cost(uint32_t tile_n, uint32_t kblocks) {
+    return std::max(kblocks * std::max((tile_n + 128) / 384.0, 0.6) + 1.5, 5.0 * tile_n / 256.0 + 1.0);
+}
+// Columns of a tile: as many as the shape allows, unless narrower tiles fill the rounds of the persistent grid better
+// (1000 x 10007 x 1024: 160 tiles of 256 x 256 on 74 pairs take three rounds, 212 of 256 x 192 three shorter ones).
+static uint32_t pick_n(uint32_t most, uint32_t least, int cg, uint32_t m, uint32_t n, uint32_t kblocks, int sms) {
+    const uint32_t groups = (uint32_t)std::max(1, sms / cg), tiles_m = ceil_div(m, 128 * (uint32_t)cg);
+    uint32_t best = most;
+    double best_cost = 1e300;
+    for (uint32_t w = most; w >= least; w -= 32) {
+        const double cost = (double)(((uint64_t)tiles_m * ceil_div(n, w) + groups - 1) / groups) * tile_cost(w, kblocks);
+        if (cost < best_cost * 0.97) { best_cost = cost; best = w; }
+    }
+    return best;
+}
+
+// One product C[m][n] = sum over k of A B^T on one shape: its tensor maps and tiles, K cut into at most `splits` parts.
+// K-major operands are stored rows x K, MN-major ones K x rows.
+struct Product {
+    CUtensorMap a, b, out;
+    Grid grid;
+};
+template <class S, bool AMN, class Epi>
+static int make_product(Product *p, const Operand &a, const Operand &b, uint32_t m, uint32_t n, uint32_t k, uint32_t splits, uint32_t tile_n,
+                        const typename Epi::Args &epi) {
+    AP_TRY(make_map_2d(&p->a, S::KIND, a.base, a.rows, a.cols, a.ld, AMN ? 64 : 128));
+    AP_TRY(make_map_2d(&p->b, S::KIND, b.base, b.rows, b.cols, b.ld, S::BMN ? 64 : tile_n / S::CG));
+    Grid &g = p->grid;
     g.tiles_m = ceil_div(m, S::M);
-    g.tiles_n = ceil_div(n, S::N);
+    g.tile_n = tile_n;
+    g.tiles_n = ceil_div(n, tile_n);
     g.kblocks = ceil_div(k, S::K);
     g.kper = ceil_div(g.kblocks, splits);
-    g.total = g.tiles_m * g.tiles_n * ceil_div(g.kblocks, g.kper);
-    AP_TRY(out_map_of(&mo, epi, ceil_div(g.kblocks, g.kper), static_cast<const Epi *>(nullptr)));
+    const uint32_t parts = ceil_div(g.kblocks, g.kper);
+    g.total = g.tiles_m * g.tiles_n * parts;
+    AP_TRY(out_map_of(&p->out, epi, parts, static_cast<const Epi *>(nullptr)));
     // row tiles that walk the columns together: all of them while their operand stays in L2 (32 MB of it), else 8
     const uint64_t row_bytes = (uint64_t)S::M * k * (S::SCALED ? 1 : 2);
     g.group_m = std::min<uint32_t>(g.tiles_m, (uint32_t)std::max<uint64_t>(8, (32ull << 20) / row_bytes));
+    return AP_OK;
+}
+template <class S, class Epi, class Epi2>
+static int tile_launch(const Product &p, uint32_t total, const Scales &sc, const typename Epi::Args &epi, const tile::Second<Epi2> &second, int sms,
+                       uint32_t *err, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};    // devices on which this kernel's shared-memory size has been set
     int device = 0;
     AP_CUDA(cudaGetDevice(&device));
     if (device >= 64 || !(allowed.load(std::memory_order_acquire) >> device & 1)) {
-        AP_CUDA(cudaFuncSetAttribute(tile::tile_kernel<S, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
+        AP_CUDA(cudaFuncSetAttribute(tile::tile_kernel<S, Epi, Epi2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
         if (device < 64) allowed.fetch_or(1ull << device, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(std::min<uint32_t>(g.total, (uint32_t)sms / S::CG) * S::CG);
+    cfg.gridDim = dim3(std::min<uint32_t>(total, std::max(1u, (uint32_t)sms / S::CG)) * S::CG);
     cfg.blockDim = dim3(tile::kThreads);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
@@ -588,8 +619,15 @@ static int tile_launch(const Operand &a, const Operand &b, uint32_t m, uint32_t 
     attr[1].val.clusterDim.x = S::CG; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    AP_CUDA(cudaLaunchKernelEx(&cfg, tile::tile_kernel<S, Epi>, ma, mb, mo, g, sc, epi, err));
+    AP_CUDA(cudaLaunchKernelEx(&cfg, tile::tile_kernel<S, Epi, Epi2>, p.a, p.b, p.out, p.grid, sc, epi, second, err));
     return AP_OK;
+}
+template <class S, class Epi>
+static int run_product(const Operand &a, const Operand &b, uint32_t m, uint32_t n, uint32_t k, uint32_t tile_n, const Scales &sc,
+                       const typename Epi::Args &epi, int sms, uint32_t *err, cudaStream_t st) {
+    Product p = {};
+    AP_TRY((make_product<S, S::AMN, Epi>(&p, a, b, m, n, k, 1, tile_n, epi)));
+    return tile_launch<S, Epi, tile::NoSecond>(p, p.grid.total, sc, epi, tile::Second<tile::NoSecond>{}, sms, err, st);
 }
 
 // SM count and address of the error word, looked up once per device
@@ -618,38 +656,63 @@ constexpr uint32_t kTileN = 256;
 static size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
 
 struct ForwardPlan { uint32_t piece, parts; size_t part_bytes, bytes; };
-// The tiles' maxima and sums (8 bytes per row and 128 columns) of at most 64 MB of documents at a time
+// narrow tiles only where few documents leave SMs without work: the partial results of a row grow with their number
+static uint32_t least_n(uint32_t docs) { return docs <= 16384 ? 32 : 128; }
+// The tiles' maxima and sums (8 bytes per row and half a tile) of at most 64 MB of documents at a time
 static ForwardPlan forward_plan(uint32_t rows, uint32_t docs) {
     ForwardPlan p;
-    const uint64_t fit = (64ull << 20) / ((uint64_t)rows * 16) * kTileN;
+    const uint32_t least = least_n(docs);
+    const uint64_t fit = (64ull << 20) / ((uint64_t)rows * 16) * least;
     p.piece = (uint32_t)std::min<uint64_t>((uint64_t)ceil_div(docs, kTileN) * kTileN, std::max<uint64_t>(fit, 32 * kTileN));
-    p.parts = 2 * ceil_div(std::min(p.piece, docs), kTileN);
+    p.parts = 2 * ceil_div(std::min(p.piece, docs), least);
     p.part_bytes = round256((size_t)rows * p.parts * 8);
     p.bytes = p.part_bytes + round256((size_t)rows * 8);
     return p;
 }
 
-struct BackwardPlan { uint32_t piece, splits; size_t ldx, ldg, ldp, x_off, g_off, p_off, bytes; };
+// The two products of a piece's gradients share a launch: the parts of dX (K = the piece's documents, cut into `splits`), then
+// the tiles of dW (K = the rows), dealt out to the groups of SMs in turn.  The cost of the group with the most work.
+struct Cut { uint32_t splits, nx, nw; };   // parts of dX's K; columns of a tile of dX and of dW
+static double pair_cost(uint32_t groups, uint32_t tx, uint32_t tw, double cx, double cw) {
+    const uint32_t rest = tx % groups;
+    const auto of = [&](uint32_t g) {
+        const uint32_t all = g < tx + tw ? (tx + tw - g - 1) / groups + 1 : 0, x = g < tx ? (tx - g - 1) / groups + 1 : 0;
+        return x * cx + (all - x) * cw;
+    };
+    return std::max(of(0), of(rest));
+}
+static Cut pick_cut(uint32_t rows, uint32_t docs, uint32_t dim, uint32_t most_splits, int sms) {
+    const uint32_t cg = rows <= 128 ? 1 : 2, groups = std::max(1u, (uint32_t)sms / cg);
+    const uint32_t mx = ceil_div(rows, 128 * cg), mw = ceil_div(docs, 128 * cg), kx = ceil_div(docs, 64), kw = ceil_div(rows, 64);
+    // the narrowest tiles that still cover dim in as few columns of tiles as the widest do
+    const uint32_t wide = ceil_div(dim, 256), n = std::max(32u, ceil_div(ceil_div(dim, wide), 32) * 32);
+    Cut best{1, n, n};
+    double best_cost = 1e300;
+    for (uint32_t s = 1; s <= most_splits && (s == 1 || kx / s >= 8); ++s) {
+        const uint32_t kper = ceil_div(kx, s);
+        if (ceil_div(kx, kper) != s) continue;
+        // every part also is a matrix of sums that is written, added to and read again
+        const double cost = pair_cost(groups, mx * wide * s, mw * wide, tile_cost(n, kper), tile_cost(n, kw)) + 0.5 * (s - 1) * mx * wide / groups;
+        if (cost < best_cost * 0.98) { best_cost = cost; best.splits = s; }
+    }
+    return best;
+}
+
+struct BackwardPlan { uint32_t piece, splits; bool direct; size_t ldx, ldg, ldp, x_off, g_off, p_off, bytes; };
 static BackwardPlan backward_plan(uint32_t rows, uint32_t docs, uint32_t dim, int sms) {
     BackwardPlan p;
-    const uint32_t pairs = std::max(1, sms / 2);
-    const uint32_t mt = ceil_div(rows, 256), nd = ceil_div(dim, 256);
-    // documents per piece: G of about 128 MB, at least 2048 documents, whole rounds of tiles in the two large products
+    // documents per piece: G of about 128 MB, at least 2048 documents
     const uint64_t most = std::max<uint64_t>(8, (128ull << 20) / ((uint64_t)rows * 2) / kTileN);
-    uint32_t best = (uint32_t)std::min<uint64_t>(most, ceil_div(docs, kTileN));
-    p.piece = best * kTileN;
+    p.piece = (uint32_t)std::min<uint64_t>(most, ceil_div(docs, kTileN)) * kTileN;
+    p.splits = pick_cut(rows, std::min(p.piece, docs), dim, 32, sms).splits;
+    p.direct = p.splits == 1 && p.piece >= docs;     // one part of one piece: dX needs no sums of its own
     p.ldx = (dim + 7) / 8 * 8;
     p.ldg = p.piece;
     p.ldp = (dim + 3) / 4 * 4;
-    // dX contracts over the documents of a piece: few tiles and a long K, so K is split until every pair of SMs has a tile
-    const uint32_t kb = ceil_div(std::min(p.piece, docs), 64);
-    const uint32_t tiles = (rows <= 128 ? ceil_div(rows, 128) : mt) * nd, units = rows <= 128 ? (uint32_t)sms : pairs;
-    p.splits = std::max<uint32_t>(1, std::min<uint32_t>(units / tiles, kb / 8));
-    p.splits = ceil_div(kb, ceil_div(kb, p.splits));
     p.x_off = 256;
     p.g_off = p.x_off + round256((size_t)rows * p.ldx * 2);
     p.p_off = p.g_off + round256((size_t)rows * p.ldg * 2);
-    p.bytes = p.p_off + round256((size_t)p.splits * rows * p.ldp * 4);
+    p.bytes = p.p_off + (p.direct ? 0 : round256((size_t)p.splits * rows * p.ldp * 4));
     return p;
 }
 
@@ -672,8 +735,9 @@ static int forward_run(const LossCall &c, const ForwardPlan &p, uint8_t *ws, flo
     for (uint32_t v0 = 0; v0 < c.docs; v0 += p.piece) {
         const uint32_t n = std::min(p.piece, c.docs - v0);
         const Operand w{static_cast<const T *>(c.w) + (size_t)v0 * c.ldw, n, c.dim, c.ldw};
-        LseEpi::Args ea{part, c.target, 2 * ceil_div(n, kTileN), c.rows, n, v0, c.scale * kLog2e};
-        AP_TRY((tile_launch<S, LseEpi>(x, w, c.rows, n, c.dim, 1, Scales{}, ea, c.sms, c.err, c.st)));
+        const uint32_t tn = pick_n(kTileN, least_n(c.docs), CG, c.rows, n, ceil_div(c.dim, 64), c.sms);
+        LseEpi::Args ea{part, c.target, 2 * ceil_div(n, tn), c.rows, n, v0, c.scale * kLog2e};
+        AP_TRY((run_product<S, LseEpi>(x, w, c.rows, n, c.dim, tn, Scales{}, ea, c.sms, c.err, c.st)));
         JoinArgs ja{part, carry, c.x, c.w, c.ldx, c.ldw, c.target, loss, lse, c.rows, c.docs, c.dim, ea.parts, v0 == 0 ? 1u : 0u,
                     v0 + n == c.docs ? 1u : 0u, c.scale};
         AP_TRY(launch(loss_join_kernel<T>, ceil_div(c.rows, 8), ja, c.st));
@@ -681,13 +745,23 @@ static int forward_run(const LossCall &c, const ForwardPlan &p, uint8_t *ws, flo
     return AP_OK;
 }
 
+// dX (stored by E: sums of parts, or the gradient itself) and dW of one piece in one launch
+template <class S, class E, class T>
+static int gradients_launch(const LossCall &c, const Cut &cut, const Operand &x, const Operand &w, const Operand &g, uint32_t n,
+                            const typename E::Args &xa, const typename StoreEpi<T>::Args &wa) {
+    Product px = {}, pw = {};
+    AP_TRY((make_product<S, false, E>(&px, g, w, c.rows, c.dim, n, cut.splits, cut.nx, xa)));
+    AP_TRY((make_product<S, true, StoreEpi<T>>(&pw, g, x, n, c.dim, c.rows, 1, cut.nw, wa)));
+    const tile::Second<StoreEpi<T>> second{pw.a, pw.b, pw.out, pw.grid, wa};
+    return tile_launch<S, E, StoreEpi<T>>(px, px.grid.total + pw.grid.total, Scales{}, xa, second, c.sms, c.err, c.st);
+}
+
 template <class T, int CG>
 static int backward_run(const LossCall &c, const BackwardPlan &p, uint8_t *ws, const float *loss, const float *lse, const float *grad, void *dx,
                         uint64_t lddx, void *dw, uint64_t lddw) {
     constexpr int KIND = Half16<T>::kind;
     using SG = tile::Shape<KIND, CG, kTileN>;                       // G: rows x documents, over dim
-    using SX = tile::Shape<KIND, CG, kTileN, false, true>;          // dX: rows x dim, over documents
-    using SW = tile::Shape<KIND, 2, kTileN, true, true>;            // dW: documents x dim, over rows
+    using SX = tile::Shape<KIND, CG, kTileN, false, true>;          // dX: rows x dim, over documents (dW: A MN-major as well)
     float *factor = reinterpret_cast<float *>(ws);
     T *xc = reinterpret_cast<T *>(ws + p.x_off), *g = reinterpret_cast<T *>(ws + p.g_off);
     float *part = reinterpret_cast<float *>(ws + p.p_off);
@@ -701,16 +775,22 @@ static int backward_run(const LossCall &c, const BackwardPlan &p, uint8_t *ws, c
         typename GradEpi<T>::Args ga{};
         ga.out.out = g; ga.out.ld = p.ldg; ga.out.m = c.rows; ga.out.n = n; ga.out.alpha = 1.f; ga.out.tma = 1; ga.out.padded = 1;
         ga.target = c.target; ga.loss = loss; ga.lse = lse; ga.grad = grad; ga.factor = factor; ga.col0 = v0; ga.docs = c.docs; ga.c = c.scale * kLog2e;
-        AP_TRY((tile_launch<SG, GradEpi<T>>(x, w, c.rows, n, c.dim, 1, Scales{}, ga, c.sms, c.err, c.st)));
+        const uint32_t tn = pick_n(kTileN, 32, CG, c.rows, n, ceil_div(c.dim, 64), c.sms);
+        AP_TRY((run_product<SG, GradEpi<T>>(x, w, c.rows, n, c.dim, tn, Scales{}, ga, c.sms, c.err, c.st)));
         typename StoreEpi<T>::Args wa{};
         wa.out = static_cast<T *>(dw) + (size_t)v0 * lddw; wa.ld = lddw; wa.m = n; wa.n = c.dim; wa.alpha = 1.f; wa.alpha_dev = factor + 1;
         wa.tma = aligned(wa.out, lddw * 2, 16);
-        AP_TRY((tile_launch<SW, StoreEpi<T>>(go, x, n, c.dim, c.rows, 1, Scales{}, wa, c.sms, c.err, c.st)));
+        Cut cut = pick_cut(c.rows, n, c.dim, p.splits, c.sms);
+        if (v0 == 0) cut.splits = p.splits;                         // the first piece writes every part, the others add to some
+        if (p.direct) {
+            typename StoreEpi<T>::Args xa{};
+            xa.out = static_cast<T *>(dx); xa.ld = lddx; xa.m = c.rows; xa.n = c.dim; xa.alpha = 1.f; xa.alpha_dev = factor + 1;
+            xa.tma = aligned(dx, lddx * 2, 16);
+            return gradients_launch<SX, StoreEpi<T>, T>(c, cut, x, w, go, n, xa, wa);
+        }
         typename StoreEpi<float>::Args xa{};
         xa.out = part; xa.ld = p.ldp; xa.m = c.rows; xa.n = c.dim; xa.alpha = 1.f; xa.add = v0 != 0; xa.tma = 1; xa.padded = 1;
-        // a short last piece has fewer splits, the first of them; without enough K blocks for each, one
-        const uint32_t splits = ceil_div(n, 64) < p.splits ? 1 : p.splits;
-        AP_TRY((tile_launch<SX, StoreEpi<float>>(go, w, c.rows, c.dim, n, splits, Scales{}, xa, c.sms, c.err, c.st)));
+        AP_TRY((gradients_launch<SX, StoreEpi<float>, T>(c, cut, x, w, go, n, xa, wa)));
     }
     FinishArgs fa{part, factor, dx, p.ldp, lddx, c.rows, c.dim, p.splits};
     const uint64_t quads = (uint64_t)c.rows * ((c.dim + 3) / 4);
@@ -727,16 +807,13 @@ static int scores_run(const ap_scaled_rows &a, const ap_scaled_rows &b, uint32_t
     ea.out = out; ea.ld = ldo; ea.m = a.rows; ea.n = b.rows; ea.alpha = alpha; ea.tma = aligned(out, ldo * sizeof(T), 16);
     const Scales sc{a.scale, b.scale, a.ld_scale, b.ld_scale, a.rows, b.rows,
                     aligned(a.scale, a.ld_scale, 4) && aligned(b.scale, b.ld_scale, 4)};
-    return tile_launch<S, StoreEpi<T>>(oa, ob, a.rows, b.rows, dim, 1, sc, ea, sms, err, st);
+    return run_product<S, StoreEpi<T>>(oa, ob, a.rows, b.rows, dim, pick_n(N, 32, CG, a.rows, b.rows, ceil_div(dim, 128), sms), sc, ea, sms, err, st);
 }
 template <class T>
 static int scores_pick(const ap_scaled_rows &a, const ap_scaled_rows &b, uint32_t dim, float alpha, void *out, uint64_t ldo, int sms, uint32_t *err,
                        cudaStream_t st) {
     T *o = static_cast<T *>(out);
-    if (a.rows > 128) return scores_run<T, 2, 224>(a, b, dim, alpha, o, ldo, sms, err, st);
-    // few rows: one CTA per tile, and narrow tiles while wide ones would leave SMs without any
-    if (ceil_div(b.rows, 224) >= (uint32_t)sms) return scores_run<T, 1, 224>(a, b, dim, alpha, o, ldo, sms, err, st);
-    return scores_run<T, 1, 64>(a, b, dim, alpha, o, ldo, sms, err, st);
+    return a.rows > 128 ? scores_run<T, 2, 224>(a, b, dim, alpha, o, ldo, sms, err, st) : scores_run<T, 1, 224>(a, b, dim, alpha, o, ldo, sms, err, st);
 }
 
 static int check_loss(const char *what, uint32_t rows, uint32_t docs, uint32_t dim, uint32_t type, const void *x, uint64_t ldx, const void *w, uint64_t ldw,

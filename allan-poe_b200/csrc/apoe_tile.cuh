@@ -18,6 +18,8 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "apoe_common.cuh"
 
 namespace apoe {
@@ -35,14 +37,15 @@ constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr int kEpiWarps = 8;                      // two per quarter of the tensor-memory lanes, each half of the columns
 constexpr int kThreads = (kEpiWarps + 4) * 32;    // + TMA producer, MMA issuer, two scale writers (e4m3 only)
 
-// One shape of the engine.  N: columns of a tile; CG: CTAs of a group; AMN / BMN: operand stored with M (N) contiguous.
+// One shape of the engine.  N: most columns of a tile (a launch may use fewer: Grid::tile_n); CG: CTAs of a group; AMN / BMN:
+// operand stored with M (N) contiguous.
 template <int KIND_, int CG_, int N_, bool AMN_ = false, bool BMN_ = false>
 struct Shape {
     static constexpr int KIND = KIND_, CG = CG_, N = N_;
     static constexpr bool AMN = AMN_, BMN = BMN_, SCALED = KIND_ == kE4m3;
     static constexpr int M = 128 * CG;
     static constexpr int K = SCALED ? 128 : 64;            // values of K in a stage: one 128-byte span
-    static constexpr int BR = N / CG;                      // rows of B a CTA loads
+    static constexpr int BR = N / CG;                      // rows of B a CTA has room for
     static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BR * 128;
     static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr uint32_t EPI_BYTES = kEpiWarps * 4096;
@@ -59,17 +62,19 @@ struct Shape {
     static_assert(BR % 8 == 0 && (!BMN || BR % 64 == 0), "rows of B per CTA");
     static_assert(!SCALED || (!AMN && !BMN), "8-bit operands are K-major");
     static_assert(N % 32 == 0 && N <= 256, "columns");
-    // kind::f16: D fp32 (bit 4), A / B type (bits 7, 10), MN-major flags (15, 16), N >> 3 (17), M >> 4 (24);
+    static_assert(!SCALED || 4 + N / 32 <= 12, "scale words");
+    // kind::f16: D fp32 (bit 4), A / B type (bits 7, 10), MN-major flags (15, 16), N >> 3 (17: added), M >> 4 (24);
     // kind::mxf8f6f4: e4m3 types are 0, scale type ue8m0 (bit 23), the byte of the scale words to use (bits 4 and 29: added)
-    static constexpr uint32_t IDESC = SCALED ? ((1u << 23) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24))
+    static constexpr uint32_t IDESC = SCALED ? ((1u << 23) | ((uint32_t)(M >> 4) << 24))
                                              : ((1u << 4) | ((uint32_t)KIND << 7) | ((uint32_t)KIND << 10) | ((AMN ? 1u : 0u) << 15) |
-                                                ((BMN ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24));
+                                                ((BMN ? 1u : 0u) << 16) | ((uint32_t)(M >> 4) << 24));
 };
 
 // The tiles of one product and their order.  Groups of `group_m` row tiles walk the column tiles together, so the tiles in
 // flight share both operands in L2.  K may be cut: split s contracts K blocks s * kper .. into a result of its own.
 struct Grid {
     uint32_t tiles_m, tiles_n, group_m, kblocks, kper, total;   // kper: K blocks of a split (the last one may have fewer)
+    uint32_t tile_n;                                            // columns of a tile: a multiple of 32, at most the shape's N
 };
 __device__ __forceinline__ void locate(const Grid &g, uint32_t id, uint32_t &mi, uint32_t &ni, uint32_t &si) {
     const uint32_t per = g.tiles_m * g.tiles_n;
@@ -226,22 +231,50 @@ struct Scales {
     uint32_t words;            // both: rows on 4-byte boundaries
 };
 
+// A warp's 4 KB of shared memory for results on their way out: two boxes of 2 KB, used in turn.
+struct Staging {
+    uint8_t *base;
+    uint32_t boxes;            // boxes written so far
+};
+
 // ---- the kernel --------------------------------------------------------------------------------------------------------
-// Epi: a type with `Args`, `Epi(const Args &, uint8_t *staging, const CUtensorMap *out, int lane)`, `begin(first row, first
+// Epi: a type with `Args`, `Epi(const Args &, Staging &, const CUtensorMap *out, int lane)`, `begin(first row, first
 // column, split, part)`, `chunk(uint32_t (&r)[32], col)` for 32 columns of the lane's row, `end()` after a tile, `finish()`
 // after the last.  Every lane of a warp makes the same calls.
-template <class S, class Epi>
+// Epi2 other than NoSecond: tiles from grid.total on belong to a second product of the same shape but for an MN-major A, with
+// operands, grid and results of its own (the two products of a gradient share one launch and fill each other's last round).
+struct NoSecond {
+    struct Args {};
+    __device__ __forceinline__ NoSecond(const Args &, Staging &, const CUtensorMap *, int) {}
+    __device__ __forceinline__ void begin(uint32_t, uint32_t, uint32_t, uint32_t) {}
+    __device__ __forceinline__ void chunk(uint32_t (&)[32], uint32_t) {}
+    __device__ __forceinline__ void end() {}
+    __device__ __forceinline__ void finish() {}
+};
+template <class Epi2>
+struct Second {
+    CUtensorMap map_a, map_b, map_out;
+    Grid grid;
+    typename Epi2::Args epi;
+};
+template <> struct Second<NoSecond> { NoSecond::Args epi; };
+template <class S, class Epi, class Epi2>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                           const __grid_constant__ CUtensorMap map_out, const Grid grid, const Scales scales, const typename Epi::Args epi_args, uint32_t *err) {
+                                                           const __grid_constant__ CUtensorMap map_out, const Grid grid, const Scales scales, const typename Epi::Args epi_args,
+                                                           const __grid_constant__ Second<Epi2> second, uint32_t *err) {
     extern __shared__ __align__(1024) uint8_t tile_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tile_smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t full_bar[S::STAGES], empty_bar[S::STAGES], tfull_bar[2], tempty_bar[2], drain_bar;
     __shared__ uint64_t sfull_bar[S::SCALED ? S::SF_SLOTS : 1], sempty_bar[S::SCALED ? S::SF_SLOTS : 1];
     __shared__ uint32_t tmem_base_s;
     constexpr int CG = S::CG;
+    constexpr bool DUAL = !std::is_same<Epi2, NoSecond>::value;
+    static_assert(!DUAL || (!S::SCALED && !S::AMN), "second products");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
     const uint32_t group = blockIdx.x / CG, groups = gridDim.x / CG;
+    uint32_t total = grid.total;
+    if constexpr (DUAL) total += second.grid.total;
 
     pdl_launch();
     if (tid == 0) {
@@ -273,11 +306,13 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         // products were issued at 215 cycles each (e4m3, 112 needed) and 170 (f16, 128 needed).
         uint32_t s = 0, phase = 0, issued = 0;
         bool ok = true;
-        for (uint32_t t = group; t < grid.total && ok; t += groups) {
+        auto load = [&](const CUtensorMap &ma, const CUtensorMap &mb, const Grid &gr, uint32_t t, auto amn) {
+            constexpr bool AMN = decltype(amn)::value;
+            const uint32_t br = gr.tile_n / CG, bytes = (S::A_BYTES + (S::BMN ? (br + 63) / 64 * 8192 : br * 128)) * CG;
             uint32_t mi, ni, si;
-            locate(grid, t, mi, ni, si);
-            const int m0 = (int)(mi * S::M + rank * 128), n0 = (int)(ni * S::N + rank * S::BR);
-            const uint32_t k0 = si * grid.kper, k1 = min(k0 + grid.kper, grid.kblocks);
+            locate(gr, t, mi, ni, si);
+            const int m0 = (int)(mi * S::M + rank * 128), n0 = (int)(ni * gr.tile_n + rank * br);
+            const uint32_t k0 = si * gr.kper, k1 = min(k0 + gr.kper, gr.kblocks);
             for (uint32_t kb = k0; kb < k1; ++kb) {
                 ok = wait(&empty_bar[s], phase ^ 1u, err, 30u);
                 if (!ok) break;
@@ -285,20 +320,25 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 const uint32_t bar = CG == 2 ? leader_addr(&full_bar[s]) : smem_u32(&full_bar[s]);
                 const int k = (int)(kb * S::K);
                 if (elect_one()) {
-                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], S::STAGE_BYTES * CG);
-                    if (S::AMN) {
-                        load_2d<CG>(st, &map_a, m0, k, bar);
-                        load_2d<CG>(st + 8192, &map_a, m0 + 64, k, bar);
-                    } else load_2d<CG>(st, &map_a, k, m0, bar);
-                    if (S::BMN) {
-#pragma unroll
-                        for (int j = 0; j < S::BR / 64; ++j) load_2d<CG>(st + S::A_BYTES + j * 8192, &map_b, n0 + j * 64, k, bar);
-                    } else load_2d<CG>(st + S::A_BYTES, &map_b, k, n0, bar);
+                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], bytes);
+                    if (AMN) {
+                        load_2d<CG>(st, &ma, m0, k, bar);
+                        load_2d<CG>(st + 8192, &ma, m0 + 64, k, bar);
+                    } else load_2d<CG>(st, &ma, k, m0, bar);
+                    if (S::BMN)
+                        for (uint32_t j = 0; j * 64 < br; ++j) load_2d<CG>(st + S::A_BYTES + j * 8192, &mb, n0 + (int)j * 64, k, bar);
+                    else load_2d<CG>(st + S::A_BYTES, &mb, k, n0, bar);
                 }
                 __syncwarp();
                 ++issued;
                 if (++s == S::STAGES) { s = 0; phase ^= 1u; }
             }
+        };
+        for (uint32_t t = group; t < total && ok; t += groups) {
+            if constexpr (DUAL) {
+                if (t >= grid.total) { load(second.map_a, second.map_b, second.grid, t - grid.total, std::true_type{}); continue; }
+            }
+            load(map_a, map_b, grid, t, std::integral_constant<bool, S::AMN>{});
         }
         if (!ok && rank == 0)   // copies still on their way (both CTAs') complete on these barriers
             for (uint32_t j = issued > S::STAGES ? issued - S::STAGES : 0; j < issued; ++j)
@@ -308,12 +348,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         if (rank == 0) {
             uint32_t s = 0, phase = 0, it = 0, sg = 0, sf = 0;
             bool ok = true;
-            for (uint32_t t = group; t < grid.total && ok; t += groups, ++it) {
-                const uint32_t si = grid.kper < grid.kblocks ? t / (grid.tiles_m * grid.tiles_n) : 0u;
-                const uint32_t k0 = si * grid.kper, k1 = min(k0 + grid.kper, grid.kblocks);
+            auto multiply = [&](const Grid &gr, uint32_t t, auto amn) {
+                constexpr bool AMN = decltype(amn)::value;
+                constexpr uint32_t FLAG = AMN && !S::AMN ? 1u << 15 : 0u;
+                const uint32_t si = gr.kper < gr.kblocks ? t / (gr.tiles_m * gr.tiles_n) : 0u;
+                const uint32_t k0 = si * gr.kper, k1 = min(k0 + gr.kper, gr.kblocks);
                 const uint32_t acc = it & 1u, d = tmem + acc * S::N;
                 ok = wait(&tempty_bar[acc], ((it >> 1) & 1u) ^ 1u, err, 31u);
-                if (!ok) break;
+                if (!ok) return;
                 fence_after();
                 for (uint32_t kb = k0; kb < k1; ++kb) {
                     ok = wait(&full_bar[s], phase, err, 32u);
@@ -328,8 +370,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                     }
                     fence_after();
                     const uint32_t a = smem_u32(smem) + s * S::STAGE_BYTES, b = a + S::A_BYTES;
-                    const uint64_t da = S::AMN ? desc_mn(a) : desc_k(a), db = S::BMN ? desc_mn(b) : desc_k(b);
-                    const uint32_t idesc = S::SCALED ? S::IDESC | ((kb & 3u) << 4) | ((kb & 3u) << 29) : S::IDESC;
+                    const uint64_t da = AMN ? desc_mn(a) : desc_k(a), db = S::BMN ? desc_mn(b) : desc_k(b);
+                    const uint32_t idesc = (S::SCALED ? S::IDESC | ((kb & 3u) << 4) | ((kb & 3u) << 29) : S::IDESC) | ((gr.tile_n >> 3) << 17) | FLAG;
                     if (elect_one()) {
                         if (fresh) {
                             const uint32_t w = smem_u32(smem) + S::STAGES * S::STAGE_BYTES + slot * S::SF_BYTES;
@@ -339,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                         }
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {             // the address field counts 16 bytes: 32 or 2048 bytes a step
-                            const uint64_t ia = da + kk * (S::AMN ? 128 : 2), ib = db + kk * (S::BMN ? 128 : 2);
+                            const uint64_t ia = da + kk * (AMN ? 128 : 2), ib = db + kk * (S::BMN ? 128 : 2);
                             const uint32_t add = (kb != k0 || kk != 0) ? 1u : 0u;
                             if (S::SCALED) mma_mx8<CG>(d, ia, ib, idesc, sf, sf + 4, add);
                             else mma_f16<CG>(d, ia, ib, idesc, add);
@@ -352,6 +394,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                     if (S::SCALED && (kb % 4 == 3 || kb + 1 == k1)) ++sg;
                     if (++s == S::STAGES) { s = 0; phase ^= 1u; }
                 }
+            };
+            for (uint32_t t = group; t < total && ok; t += groups, ++it) {
+                if constexpr (DUAL) {
+                    if (t >= grid.total) { multiply(second.grid, t - grid.total, std::true_type{}); continue; }
+                }
+                multiply(grid, t, std::integral_constant<bool, S::AMN>{});
             }
             if (!ok) {   // instructions in flight finish before the tensor memory is given back
                 if (elect_one()) commit<CG>(&drain_bar);
@@ -372,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             auto fetch = [&](uint32_t (&w)[ROWS]) {
                 uint32_t mi, ni, si;
                 locate(grid, t, mi, ni, si);
-                const uint32_t m0 = mi * S::M + rank * 128, n0 = ni * S::N, kb = grp * 4;
+                const uint32_t m0 = mi * S::M + rank * 128, n0 = ni * grid.tile_n, kb = grp * 4;
 #pragma unroll
                 for (int j = 0; j < ROWS; ++j) {
                     const bool of_a = j < 4;
@@ -422,21 +470,24 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         // ---------------- epilogue: warp w reads the lanes 32 (w mod 4) .. of the accumulator, warps 0-3 the first half of
         // the columns, 4-7 the second ------------------------------------------------------------------------------------
         const int quarter = warp & 3, half = warp >> 2;
-        constexpr int CHUNKS = S::N / 32, FIRST = (CHUNKS + 1) / 2;
-        Epi epi(epi_args, smem + S::STAGES * S::STAGE_BYTES + S::SF_ROOM + warp * 4096, &map_out, lane);
+        Staging staging{smem + S::STAGES * S::STAGE_BYTES + S::SF_ROOM + warp * 4096, 0u};
+        Epi epi(epi_args, staging, &map_out, lane);
+        const CUtensorMap *out2 = nullptr;
+        if constexpr (DUAL) out2 = &second.map_out;
+        Epi2 epi2(second.epi, staging, out2, lane);
         uint32_t it = 0;
         bool ok = true;
-        for (uint32_t t = group; t < grid.total && ok; t += groups, ++it) {
+        auto finish_tile = [&](const Grid &gr, uint32_t t, auto &e) {
             uint32_t mi, ni, si;
-            locate(grid, t, mi, ni, si);
-            const uint32_t acc = it & 1u;
-            epi.begin(mi * S::M + rank * 128 + quarter * 32, ni * S::N, si, ni * 2 + half);
+            locate(gr, t, mi, ni, si);
+            const int chunks = (int)gr.tile_n / 32, c0 = half ? (chunks + 1) / 2 : 0, c1 = half ? chunks : (chunks + 1) / 2;
+            const uint32_t acc = it & 1u, col = ni * gr.tile_n;
+            e.begin(mi * S::M + rank * 128 + quarter * 32, col, si, ni * 2 + half);
             ok = wait(&tfull_bar[acc], (it >> 1) & 1u, err, 34u);
             ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) break;
+            if (!ok) return;
             fence_after();
             const uint32_t src = tmem + ((uint32_t)(32 * quarter) << 16) + acc * S::N;
-            const int c0 = half ? FIRST : 0, c1 = half ? CHUNKS : FIRST;
             auto release = [&]() {          // the last read of this warp is done: the accumulator can be written again
                 fence_before();
                 __syncwarp();
@@ -446,26 +497,35 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 }
             };
             uint32_t r0[32], r1[32];        // one chunk is worked on while the next one is read
-            tmem_ld32(r0, src + c0 * 32);
-            tmem_wait_ld();
-            if (c1 - c0 == 1) release();
+            if (c0 < c1) {
+                tmem_ld32(r0, src + c0 * 32);
+                tmem_wait_ld();
+            }
+            if (c1 - c0 <= 1) release();
             for (int c = c0; c < c1; c += 2) {
                 if (c + 1 < c1) tmem_ld32(r1, src + (c + 1) * 32);
-                epi.chunk(r0, ni * S::N + c * 32);
+                e.chunk(r0, col + c * 32);
                 if (c + 1 < c1) {
                     tmem_wait_ld();
                     if (c + 2 < c1) tmem_ld32(r0, src + (c + 2) * 32);
                     else release();
-                    epi.chunk(r1, ni * S::N + (c + 1) * 32);
+                    e.chunk(r1, col + (c + 1) * 32);
                     if (c + 2 < c1) {
                         tmem_wait_ld();
                         if (c + 3 >= c1) release();
                     }
                 }
             }
-            epi.end();
+            e.end();
+        };
+        for (uint32_t t = group; t < total && ok; t += groups, ++it) {
+            if constexpr (DUAL) {
+                if (t >= grid.total) { finish_tile(second.grid, t - grid.total, epi2); continue; }
+            }
+            finish_tile(grid, t, epi);
         }
         epi.finish();
+        epi2.finish();
     }
     fence_before();
     __syncthreads();
