@@ -80,85 +80,88 @@ struct QuantArgs {
     const void *src;
     uint8_t *q, *scale;
     size_t lds, ldq, ldsc;     // row strides: elements of src, bytes of q and scale
-    uint32_t items;            // rows x blocks
+    uint32_t items;            // rows x blocks, below 2^31
     uint32_t dim, blocks;
-    uint32_t vec;              // src and q rows allow 16-byte loads and the stores that go with them
+    uint32_t magic, shift;     // item / blocks = umulhi(item, magic) >> shift, for items below 2^31
 };
 
-// One pass, bound by memory.  A lane holds 16 bytes of a block: the 32 lanes of a warp one block of f32, two blocks of f16 or
-// bf16; shuffles give each block's maximum.  A warp has four such loads in flight, of neighbouring blocks.
+// One pass, bound by memory where the arithmetic of rows stays small.  A lane holds 16 bytes of a block: the 32 lanes of a warp
+// one block of f32, two blocks of f16 or bf16; shuffles give each block's maximum.  A warp has four such loads in flight, of
+// neighbouring blocks; one round per warp (a persistent grid with the next round's loads ahead of the current one's work was
+// slower: 217 to 281 us instead of 149 for 200 000 x 1024 f32, by its registers).
+//   kFlat: whole blocks, rows back to back on both sides: the matrix is one row of blocks (6.9 TB/s at 200 000 x 1024 f32)
+//   kUnits: rows of whole 16-byte units on 16-byte boundaries;  kAny: the rest, value by value where it has to be
+enum : int { kFlat, kUnits, kAny };
 constexpr int kQuantUnroll = 4;
-template <class T>
+template <class T, int MODE>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantArgs a) {
     constexpr int V = 16 / (int)sizeof(T), LANES = 128 / V, PER = 32 / LANES;   // values of a lane, lanes and blocks of a load
     constexpr uint32_t STEP = kQuantUnroll * PER;
     const uint32_t lane = threadIdx.x & 31, sub = lane / LANES, c0 = (lane % LANES) * V;
-    const uint32_t warps = gridDim.x * (blockDim.x >> 5), warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const uint32_t warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     tile::pdl_launch();
     tile::pdl_wait();
-    const uint32_t rounds = (a.items - 1) / STEP + 1;
-    for (uint32_t round = warp; round < rounds; round += warps) {
-        uint32_t row[kQuantUnroll], blk[kQuantUnroll];
-        bool live[kQuantUnroll];
-        uint4 raw[kQuantUnroll];
-        const uint32_t it0 = round * STEP + sub;
-        uint32_t r = it0 / a.blocks, b = it0 - r * a.blocks;
+    const uint32_t it0 = warp * STEP + sub;
+    uint32_t row[kQuantUnroll], c[kQuantUnroll];      // first value of the lane: row, and place in it (kFlat: block, 0)
+    uint4 raw[kQuantUnroll];
+    auto live = [&](int u) { return it0 + u * PER < a.items; };
 #pragma unroll
-        for (int u = 0; u < kQuantUnroll; ++u) {
-            live[u] = it0 + u * PER < a.items && it0 + u * PER >= it0;
-            row[u] = r; blk[u] = b;
-            b += PER;
-            while (b >= a.blocks) { b -= a.blocks; ++r; }
-            raw[u] = make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t c = blk[u] * 128 + c0;
-            if (live[u] && c < a.dim) {
-                const T *p = static_cast<const T *>(a.src) + (size_t)row[u] * a.lds + c;
-                if (a.vec && c + V <= a.dim) raw[u] = __ldcs(reinterpret_cast<const uint4 *>(p));
-                else {
-                    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    for (int u = 0; u < kQuantUnroll; ++u) {
+        const uint32_t it = it0 + u * PER;
+        row[u] = MODE == kFlat || a.blocks == 1 ? it : __umulhi(it, a.magic) >> a.shift;
+        c[u] = (MODE == kFlat ? 0u : (it - row[u] * a.blocks) * 128) + c0;
+        raw[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (!live(u) || (MODE != kFlat && c[u] >= a.dim)) continue;
+        const T *p = static_cast<const T *>(a.src) + (size_t)row[u] * (MODE == kFlat ? 128 : a.lds) + c[u];
+        if (MODE != kAny) raw[u] = __ldcs(reinterpret_cast<const uint4 *>(p));
+        else {
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (c + i < a.dim) {
-                            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
-                            else w[i / 2] |= (uint32_t)*reinterpret_cast<const uint16_t *>(p + i) << (16 * (i & 1));
-                        }
-                    raw[u] = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int i = 0; i < V; ++i)
+                if (c[u] + i < a.dim) {
+                    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
+                    else w[i / 2] |= (uint32_t)*reinterpret_cast<const uint16_t *>(p + i) << (16 * (i & 1));
                 }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kQuantUnroll; ++u) {
-            float v[V];
-            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
-                else { const float2 f = Half16<T>::unpack(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
-            }
-            float m = 0.0f;                                  // a NaN is never taken: fmaxf returns the other one
-#pragma unroll
-            for (int i = 0; i < V; ++i) m = fmaxf(m, fabsf(v[i]));
-#pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
-            const int e = block_exponent(m);
-            const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-            const uint32_t c = blk[u] * 128 + c0;
-            if (!live[u] || c >= a.dim) continue;
-            uint32_t p[V / 4];
-#pragma unroll
-            for (int i = 0; i < V / 4; ++i)
-                p[i] = e4m3x2(v[4 * i] * down, v[4 * i + 1] * down) | (e4m3x2(v[4 * i + 2] * down, v[4 * i + 3] * down) << 16);
-            uint8_t *o = a.q + (size_t)row[u] * a.ldq + c;
-            if (a.vec && c + V <= a.dim) {
-                if constexpr (V == 4) *reinterpret_cast<uint32_t *>(o) = p[0];
-                else *reinterpret_cast<uint2 *>(o) = make_uint2(p[0], p[1]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) if (c + i < a.dim) o[i] = (uint8_t)(p[i / 4] >> (8 * (i & 3)));
-            }
-            if (c0 == 0) a.scale[(size_t)row[u] * a.ldsc + blk[u]] = (uint8_t)(e + 127);
+            raw[u] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
+    uint8_t mine = 0, *at = nullptr;
+#pragma unroll
+    for (int u = 0; u < kQuantUnroll; ++u) {
+        float v[V];
+        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+            else { const float2 f = Half16<T>::unpack(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+        }
+        float m = 0.0f;                                  // a NaN is never taken: fmaxf returns the other one
+#pragma unroll
+        for (int i = 0; i < V; ++i) m = fmaxf(m, fabsf(v[i]));
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+        const int e = block_exponent(m);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        if (!live(u)) continue;
+        if (lane % LANES == (uint32_t)u) {
+            mine = (uint8_t)(e + 127);
+            at = a.scale + (MODE == kFlat ? row[u] : (size_t)row[u] * a.ldsc + c[u] / 128);
+        }
+        if (MODE != kFlat && c[u] >= a.dim) continue;
+        uint32_t p[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+            p[i] = e4m3x2(v[4 * i] * down, v[4 * i + 1] * down) | (e4m3x2(v[4 * i + 2] * down, v[4 * i + 3] * down) << 16);
+        uint8_t *o = a.q + (size_t)row[u] * (MODE == kFlat ? 128 : a.ldq) + c[u];
+        if (MODE != kAny) {
+            if constexpr (V == 4) *reinterpret_cast<uint32_t *>(o) = p[0];
+            else *reinterpret_cast<uint2 *>(o) = make_uint2(p[0], p[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) if (c[u] + i < a.dim) o[i] = (uint8_t)(p[i / 4] >> (8 * (i & 3)));
+        }
+    }
+    if (at) *at = mine;      // the scale bytes of the warp's blocks in one store
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -234,10 +237,14 @@ struct StoreEpi {
                 const uint32_t rows = min(32u, a.m - row0);
                 constexpr int PER = 16 / (int)sizeof(T), RPI = 32 / COLS;      // values of a unit, rows a pass covers
                 const int k = lane % COLS;
-                if (c + k < a.n)
-                    for (uint32_t row = lane / COLS; row < rows; row += RPI)
-                        a.out[(size_t)(row0 + row) * a.ld + c + k] =
-                            *reinterpret_cast<const T *>(box + row * 64 + (((k / PER) ^ ((row >> 1) & 3)) << 4) + (k % PER) * sizeof(T));
+                T *o = a.out + (size_t)row0 * a.ld + c + k;
+                const bool in = c + k < a.n;
+#pragma unroll 8
+                for (int i = 0; i < 32 / RPI; ++i) {
+                    const uint32_t row = i * RPI + lane / COLS;
+                    const T v = *reinterpret_cast<const T *>(box + row * 64 + (((k / PER) ^ ((row >> 1) & 3)) << 4) + (k % PER) * sizeof(T));
+                    if (in && row < rows) o[(size_t)row * a.ld] = v;
+                }
                 __syncwarp();
             }
         }
@@ -856,21 +863,27 @@ extern "C" int ap_quantize_rows_device(int device, uint32_t rows, uint32_t dim, 
     if (!src || !q || !scale) return fail(AP_ERR_ARG, "quantize: null argument");
     const uint32_t blocks = ceil_div(dim, 128);
     if (ld < dim || ldq < dim || ld_scale < blocks) return fail(AP_ERR_ARG, "quantize: a row stride is shorter than a row");
-    if ((uint64_t)rows * blocks >= (1ull << 32)) return fail(AP_ERR_LIMIT, "quantize: %u rows of %u blocks in one call", rows, blocks);
+    if ((uint64_t)rows * blocks >= (1ull << 31)) return fail(AP_ERR_LIMIT, "quantize: %u rows of %u blocks in one call", rows, blocks);
     if ((uintptr_t)src % (uint32_t)size) return fail(AP_ERR_ARG, "quantize: the source is not aligned to its type");
     DeviceScope scope;
     AP_TRY(scope.enter(device));
     int sms;
     uint32_t *err;
     AP_TRY(device_facts(device, &sms, &err));
-    QuantArgs a{src, q, scale, ld, ldq, ld_scale, rows * blocks, dim, blocks, 0};
-    a.vec = aligned(src, ld * size, 16) && aligned(q, ldq, 16 / size);
-    const uint32_t step = kQuantUnroll * 8 * (size == 4 ? 1 : 2);
-    const uint32_t grid = std::min<uint32_t>((a.items - 1) / step + 1, 8 * (uint32_t)sms);
+    QuantArgs a{src, q, scale, ld, ldq, ld_scale, rows * blocks, dim, blocks, 0, 0};
+    if (blocks > 1) {                  // with s = ceil(log2 blocks): magic = ceil(2^(31 + s) / blocks) < 2^32, exact for items below 2^31
+        uint32_t s = 1;
+        while ((1u << s) < blocks) ++s;
+        a.magic = (uint32_t)(((1ull << (31 + s)) + blocks - 1) / blocks);
+        a.shift = s - 1;
+    }
+    const bool units = aligned(src, ld * size, 16) && aligned(q, ldq, 16 / size) && dim % (16 / size) == 0;
+    const bool flat = units && dim % 128 == 0 && ld == dim && ldq == dim && ld_scale == blocks;
+    const uint32_t step = kQuantUnroll * 8 * (size == 4 ? 1 : 2), grid = (a.items - 1) / step + 1;
     cudaStream_t st = (cudaStream_t)stream;
-    if (type == AP_TYPE_F32) return launch(quantize_kernel<float>, grid, a, st);
-    if (type == AP_TYPE_F16) return launch(quantize_kernel<__half>, grid, a, st);
-    return launch(quantize_kernel<__nv_bfloat16>, grid, a, st);
+    if (type == AP_TYPE_F32) return launch(flat ? quantize_kernel<float, kFlat> : units ? quantize_kernel<float, kUnits> : quantize_kernel<float, kAny>, grid, a, st);
+    if (type == AP_TYPE_F16) return launch(flat ? quantize_kernel<__half, kFlat> : units ? quantize_kernel<__half, kUnits> : quantize_kernel<__half, kAny>, grid, a, st);
+    return launch(flat ? quantize_kernel<__nv_bfloat16, kFlat> : units ? quantize_kernel<__nv_bfloat16, kUnits> : quantize_kernel<__nv_bfloat16, kAny>, grid, a, st);
 }
 
 extern "C" int ap_scaled_scores_device(int device, uint32_t dim, const ap_scaled_rows *a, const ap_scaled_rows *b, float alpha, uint32_t out_type, void *out,

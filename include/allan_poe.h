@@ -357,7 +357,7 @@ int ap_dense_check_status(int device, void *stream);
  * max |x| <= 448 * 2^e, q = e4m3(x * 2^-e) to nearest even, scale byte = e + 127 (value 2^e).  A NaN becomes the e4m3 NaN and
  * does not count for the maximum; an infinity becomes +-448 with a scale whose product overflows to infinity in fp32.
  * src: rows x dim values of `type`, ld apart; q: bytes, ldq apart; scale: ceil(dim / 128) bytes per row, ld_scale apart.
- * rows = 0 does nothing. */
+ * rows = 0 does nothing; rows x ceil(dim / 128) stays below 2^31. */
 int ap_quantize_rows_device(int device, uint32_t rows, uint32_t dim, uint32_t type, const void *src, uint64_t ld, uint8_t *q,
                             uint64_t ldq, uint8_t *scale, uint64_t ld_scale, void *stream);
 typedef struct {
