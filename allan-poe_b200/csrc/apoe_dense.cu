@@ -678,28 +678,31 @@ static ForwardPlan forward_plan(uint32_t rows, uint32_t docs) {
 }
 
 // The two products of a piece's gradients share a launch: the parts of dX (K = the piece's documents, cut into `splits`), then
-// the tiles of dW (K = the rows), dealt out to the groups of SMs in turn.  The cost of the group with the most work.
-struct Cut { uint32_t splits, nx, nw; };   // parts of dX's K; columns of a tile of dX and of dW
-static double pair_cost(uint32_t groups, uint32_t tx, uint32_t tw, double cx, double cw) {
-    const uint32_t rest = tx % groups;
-    const auto of = [&](uint32_t g) {
-        const uint32_t all = g < tx + tw ? (tx + tw - g - 1) / groups + 1 : 0, x = g < tx ? (tx - g - 1) / groups + 1 : 0;
-        return x * cx + (all - x) * cw;
-    };
-    return std::max(of(0), of(rest));
+// the tiles of dW (K = the rows).  The groups of SMs that get a part of dX less get `lead` tiles of dW more.
+struct Cut { uint32_t splits, n; };        // parts of dX's K; columns of a tile
+struct Deal { uint32_t lead; double cost; };
+static Deal deal(uint32_t groups, uint32_t tx, uint32_t tw, double cx, double cw) {
+    const uint32_t each = tx / groups, rest = tx % groups, light = groups - rest;
+    const uint32_t lead = rest ? std::min<uint32_t>((uint32_t)(cx / cw + 0.5), tw / light) : 0, left = tw - lead * light;
+    const auto turns = [&](uint32_t g) { return left > g ? (left - g - 1) / groups + 1 : 0; };
+    const double heavy = rest ? (each + 1) * cx + turns(0) * cw : 0.0, lighter = each * cx + (lead + turns(rest)) * cw;
+    return {lead, std::max(heavy, lighter)};
+}
+static Deal deal_of(uint32_t rows, uint32_t docs, uint32_t dim, const Cut &c, int sms) {
+    const uint32_t cg = rows <= 128 ? 1 : 2, groups = std::max(1u, (uint32_t)sms / cg), cols = ceil_div(dim, c.n), kx = ceil_div(docs, 64);
+    const uint32_t tx = ceil_div(rows, 128 * cg) * cols * c.splits, tw = ceil_div(docs, 128 * cg) * cols;
+    return deal(std::min(groups, tx + tw), tx, tw, tile_cost(c.n, ceil_div(kx, c.splits)), tile_cost(c.n, ceil_div(rows, 64)));
 }
 static Cut pick_cut(uint32_t rows, uint32_t docs, uint32_t dim, uint32_t most_splits, int sms) {
-    const uint32_t cg = rows <= 128 ? 1 : 2, groups = std::max(1u, (uint32_t)sms / cg);
-    const uint32_t mx = ceil_div(rows, 128 * cg), mw = ceil_div(docs, 128 * cg), kx = ceil_div(docs, 64), kw = ceil_div(rows, 64);
     // the narrowest tiles that still cover dim in as few columns of tiles as the widest do
-    const uint32_t wide = ceil_div(dim, 256), n = std::max(32u, ceil_div(ceil_div(dim, wide), 32) * 32);
-    Cut best{1, n, n};
+    const uint32_t wide = ceil_div(dim, 256), kx = ceil_div(docs, 64);
+    Cut best{1, std::max(32u, ceil_div(ceil_div(dim, wide), 32) * 32)};
     double best_cost = 1e300;
     for (uint32_t s = 1; s <= most_splits && (s == 1 || kx / s >= 8); ++s) {
-        const uint32_t kper = ceil_div(kx, s);
-        if (ceil_div(kx, kper) != s) continue;
-        // every part also is a matrix of sums that is written, added to and read again
-        const double cost = pair_cost(groups, mx * wide * s, mw * wide, tile_cost(n, kper), tile_cost(n, kw)) + 0.5 * (s - 1) * mx * wide / groups;
+        if (ceil_div(kx, ceil_div(kx, s)) != s) continue;
+        const Cut c{s, best.n};
+        // a part is a matrix of fp32 sums that is written and read once more: its time at 6.5 TB/s, in units of 0.5 us
+        const double cost = deal_of(rows, docs, dim, c, sms).cost + (s > 1 ? 2.0 + s * (double)rows * dim * 6.0 / 6.5e12 / 0.5e-6 : 0.0);
         if (cost < best_cost * 0.98) { best_cost = cost; best.splits = s; }
     }
     return best;
@@ -708,8 +711,9 @@ static Cut pick_cut(uint32_t rows, uint32_t docs, uint32_t dim, uint32_t most_sp
 struct BackwardPlan { uint32_t piece, splits; bool direct; size_t ldx, ldg, ldp, x_off, g_off, p_off, bytes; };
 static BackwardPlan backward_plan(uint32_t rows, uint32_t docs, uint32_t dim, int sms) {
     BackwardPlan p;
-    // documents per piece: G of about 128 MB, at least 2048 documents
-    const uint64_t most = std::max<uint64_t>(8, (128ull << 20) / ((uint64_t)rows * 2) / kTileN);
+    // documents per piece: G of about 512 MB, at least 2048 documents (4096 x 50 021 x 1024, both gradients:
+    // 1.15 ms with 32 MB, 1.10 with 128 MB, 1.06 with 512 MB: every piece adds to the sums of dX once more)
+    const uint64_t most = std::max<uint64_t>(8, (512ull << 20) / ((uint64_t)rows * 2) / kTileN);
     p.piece = (uint32_t)std::min<uint64_t>(most, ceil_div(docs, kTileN)) * kTileN;
     p.splits = pick_cut(rows, std::min(p.piece, docs), dim, 32, sms).splits;
     p.direct = p.splits == 1 && p.piece >= docs;     // one part of one piece: dX needs no sums of its own
@@ -757,9 +761,9 @@ template <class S, class E, class T>
 static int gradients_launch(const LossCall &c, const Cut &cut, const Operand &x, const Operand &w, const Operand &g, uint32_t n,
                             const typename E::Args &xa, const typename StoreEpi<T>::Args &wa) {
     Product px = {}, pw = {};
-    AP_TRY((make_product<S, false, E>(&px, g, w, c.rows, c.dim, n, cut.splits, cut.nx, xa)));
-    AP_TRY((make_product<S, true, StoreEpi<T>>(&pw, g, x, n, c.dim, c.rows, 1, cut.nw, wa)));
-    const tile::Second<StoreEpi<T>> second{pw.a, pw.b, pw.out, pw.grid, wa};
+    AP_TRY((make_product<S, false, E>(&px, g, w, c.rows, c.dim, n, cut.splits, cut.n, xa)));
+    AP_TRY((make_product<S, true, StoreEpi<T>>(&pw, g, x, n, c.dim, c.rows, 1, cut.n, wa)));
+    const tile::Second<StoreEpi<T>> second{pw.a, pw.b, pw.out, pw.grid, deal_of(c.rows, n, c.dim, cut, c.sms).lead, wa};
     return tile_launch<S, E, StoreEpi<T>>(px, px.grid.total + pw.grid.total, Scales{}, xa, second, c.sms, c.err, c.st);
 }
 

@@ -241,8 +241,10 @@ struct Staging {
 // Epi: a type with `Args`, `Epi(const Args &, Staging &, const CUtensorMap *out, int lane)`, `begin(first row, first
 // column, split, part)`, `chunk(uint32_t (&r)[32], col)` for 32 columns of the lane's row, `end()` after a tile, `finish()`
 // after the last.  Every lane of a warp makes the same calls.
-// Epi2 other than NoSecond: tiles from grid.total on belong to a second product of the same shape but for an MN-major A, with
-// operands, grid and results of its own (the two products of a gradient share one launch and fill each other's last round).
+// Epi2 other than NoSecond: a second product of the same shape but for an MN-major A, with operands, grid and results of its
+// own, whose tiles follow the first one's (the two products of a gradient share one launch and fill each other's rounds).
+// Tiles of a product are dealt out in turn; the groups that get one tile of the first product less than the others get
+// `lead` tiles of the second before the turns begin, so all end together although the tiles differ in cost.
 struct NoSecond {
     struct Args {};
     __device__ __forceinline__ NoSecond(const Args &, Staging &, const CUtensorMap *, int) {}
@@ -255,6 +257,7 @@ template <class Epi2>
 struct Second {
     CUtensorMap map_a, map_b, map_out;
     Grid grid;
+    uint32_t lead;
     typename Epi2::Args epi;
 };
 template <> struct Second<NoSecond> { NoSecond::Args epi; };
@@ -273,8 +276,23 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
     const uint32_t group = blockIdx.x / CG, groups = gridDim.x / CG;
-    uint32_t total = grid.total;
-    if constexpr (DUAL) total += second.grid.total;
+    // this group's tiles, in order: `first(tile)` for the first product, `then(tile)` for the second, while `ok`
+    auto walk = [&](const bool &ok, auto first, auto then) {
+        for (uint32_t t = group; t < grid.total && ok; t += groups) first(t);
+        if constexpr (DUAL) {
+            const uint32_t rest = grid.total % groups, light = groups - rest, before = second.lead * light;
+            uint32_t i = 0, t = group;
+            if (group >= rest) t = second.lead ? group - rest : before + group;
+            else t = before + group;
+            while (t < second.grid.total && ok) {
+                then(t);
+                ++i;
+                if (group >= rest && i < second.lead) t += light;
+                else if (group >= rest && i == second.lead) t = before + group;
+                else t += groups;
+            }
+        }
+    };
 
     pdl_launch();
     if (tid == 0) {
@@ -334,12 +352,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 if (++s == S::STAGES) { s = 0; phase ^= 1u; }
             }
         };
-        for (uint32_t t = group; t < total && ok; t += groups) {
-            if constexpr (DUAL) {
-                if (t >= grid.total) { load(second.map_a, second.map_b, second.grid, t - grid.total, std::true_type{}); continue; }
-            }
-            load(map_a, map_b, grid, t, std::integral_constant<bool, S::AMN>{});
-        }
+        walk(ok, [&](uint32_t t) { load(map_a, map_b, grid, t, std::integral_constant<bool, S::AMN>{}); },
+             [&](uint32_t t) { if constexpr (DUAL) load(second.map_a, second.map_b, second.grid, t, std::true_type{}); });
         if (!ok && rank == 0)   // copies still on their way (both CTAs') complete on these barriers
             for (uint32_t j = issued > S::STAGES ? issued - S::STAGES : 0; j < issued; ++j)
                 wait(&full_bar[j % S::STAGES], (j / S::STAGES) & 1u, nullptr, 0u, 1u << 12);
@@ -395,12 +409,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                     if (++s == S::STAGES) { s = 0; phase ^= 1u; }
                 }
             };
-            for (uint32_t t = group; t < total && ok; t += groups, ++it) {
-                if constexpr (DUAL) {
-                    if (t >= grid.total) { multiply(second.grid, t - grid.total, std::true_type{}); continue; }
-                }
-                multiply(grid, t, std::integral_constant<bool, S::AMN>{});
-            }
+            walk(ok, [&](uint32_t t) { multiply(grid, t, std::integral_constant<bool, S::AMN>{}); ++it; },
+                 [&](uint32_t t) { if constexpr (DUAL) { multiply(second.grid, t, std::true_type{}); ++it; } });
             if (!ok) {   // instructions in flight finish before the tensor memory is given back
                 if (elect_one()) commit<CG>(&drain_bar);
                 wait(&drain_bar, 0u, nullptr, 0u, 1u << 14);
@@ -518,12 +528,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             }
             e.end();
         };
-        for (uint32_t t = group; t < total && ok; t += groups, ++it) {
-            if constexpr (DUAL) {
-                if (t >= grid.total) { finish_tile(second.grid, t - grid.total, epi2); continue; }
-            }
-            finish_tile(grid, t, epi);
-        }
+        walk(ok, [&](uint32_t t) { finish_tile(grid, t, epi); ++it; },
+             [&](uint32_t t) { if constexpr (DUAL) { finish_tile(second.grid, t, epi2); ++it; } });
         epi.finish();
         epi2.finish();
     }

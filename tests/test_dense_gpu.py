@@ -395,9 +395,11 @@ def test_certain_and_hopeless_rows_keep_their_digits():
     assert float((dq.double() - scale * (p @ d.double())).abs().max()) <= 0.02 * float(dq.abs().max())
 
 
-def test_pieces_of_the_documents_join():
-    """More rows than one piece of the workspaces covers: several pieces forward and back, the last one short."""
-    rows, docs, dim = 8192, 9000, 64
+@pytest.mark.parametrize("rows,docs", [(8192, 9000), (65000, 8461), (40001, 20011)])
+def test_pieces_of_the_documents_join(rows, docs):
+    """More rows than one piece of the workspaces covers (from 40 000 rows on): several pieces forward and back, the last one
+    short."""
+    dim = 64
     q, d, t, scale = loss_case(rows, docs, dim, torch.bfloat16, 21)
     grad = torch.full((rows,), 1.0 / rows, device=DEV)
     loss, lse = apoe.softmax_loss_forward(q, d, t, scale)
