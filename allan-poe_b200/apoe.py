@@ -522,7 +522,9 @@ def quantize_rows(x, stream=None):
 
 def scaled_scores(a, a_scale, b, b_scale, out_dtype=None, alpha: float = 1.0, out=None, stream=None):
     """Scores of 8-bit rows (as `quantize_rows` returns them): [rows of a, rows of b] in out_dtype (float32 by default,
-    float16, bfloat16), summed in fp32.  Rows of a and b must start on 16-byte boundaries."""
+    float16, bfloat16), summed in fp32.  Rows of a and b must start on 16-byte boundaries.  Without `out` the result's rows
+    start on 16-byte boundaries too (they are further apart than they are long where a row is no multiple of 16 bytes); any
+    matrix with contiguous rows is taken as `out`, rows off these boundaries are written more slowly."""
     T = _T or _torch()
     m, dim, lda = _matrix("a", a, -1, (T.f8,))
     device = a.get_device()
@@ -535,8 +537,12 @@ def scaled_scores(a, a_scale, b, b_scale, out_dtype=None, alpha: float = 1.0, ou
     if ma != m or nb != n or ca != blocks or cb != blocks:
         raise ApoeError(1, f"scores: scales {ma} x {ca} and {nb} x {cb}, needed {m} x {blocks} and {n} x {blocks}")
     if out is None:
-        out = a.new_empty((m, n), dtype=out_dtype or T.f32)
-        ldo = n
+        kind = T.types.get(out_dtype, -1) if out_dtype is not None else TYPE_F32
+        unit = 4 if kind == TYPE_F32 else 8                       # values of 16 bytes
+        ldo = (n + unit - 1) // unit * unit
+        out = a.new_empty((m, n if m == 1 else ldo), dtype=out_dtype or T.f32)
+        if ldo != n and m != 1:
+            out = out[:, :n]
     else:
         om, on, ldo = _matrix("out", out, device, T.types)
         if om != m or on != n:

@@ -194,9 +194,11 @@ struct StoreEpi {
     __device__ __forceinline__ StoreEpi(const Args &args, tile::Staging &staging, const CUtensorMap *out, int lane_) : a(args), st(staging), map(out), lane(lane_) {
         alpha = a.alpha_dev ? a.alpha * __ldg(a.alpha_dev) : a.alpha;
     }
+    __device__ __forceinline__ void ahead(uint32_t) {}
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t s, uint32_t) { row0 = r0; split = s; }
     __device__ __forceinline__ void end() {}
-    __device__ __forceinline__ void finish() { if (lane == 0) tile::store_wait_all(); }
+    // shared memory is given up when the copies have read it; that they are written is part of the kernel's end
+    __device__ __forceinline__ void finish() { if (lane == 0) tile::store_wait_read<0>(); }
     __device__ __forceinline__ void chunk(uint32_t (&r)[32], uint32_t col) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
@@ -257,6 +259,19 @@ __device__ __forceinline__ float exp2_fast(float x) {   // 2^x, 2 ulp; results b
     return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {   // a NaN is never taken
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// two fp32 operations in one instruction
+struct Pair { uint64_t v; };
+__device__ __forceinline__ Pair pair(float lo, float hi) { Pair p; asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi)); return p; }
+__device__ __forceinline__ float2 split(Pair p) { float2 f; asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v)); return f; }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { Pair d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return d; }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) { Pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) { Pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
+
 // Running maximum and sum of 2^(l log2 e) of a row over the columns of a tile, the target's column left out: the target's
 // own logit is computed on its own, in fp32 over all of K, because the loss is a difference against it.
 struct LseEpi {
@@ -268,32 +283,45 @@ struct LseEpi {
     };
     const Args &a;
     int lane;
-    uint32_t row = 0, part = 0, tgt = 0;
+    uint32_t row = 0, part = 0, tgt = 0, next = kNoTarget;
     float top = 0.f, sum = 0.f;
     __device__ __forceinline__ LseEpi(const Args &args, tile::Staging &, const CUtensorMap *, int lane_) : a(args), lane(lane_) {}
+    __device__ __forceinline__ void ahead(uint32_t r0) { next = r0 + lane < a.m ? __ldg(a.target + r0 + lane) : kNoTarget; }
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t, uint32_t p) {
         row = r0 + lane; part = p;
-        tgt = row < a.m ? __ldg(a.target + row) - a.col0 : kNoTarget;   // columns are below 2^31: no match for a target of another piece
+        tgt = next - a.col0;              // a target of another piece is none of this one's columns, and kNoTarget none at all
         top = -1.0e30f; sum = 0.f;
     }
     __device__ __forceinline__ void chunk(uint32_t (&r)[32], uint32_t col) {
-        float v[32];
+        // the maximum of l = c s is |c| times the maximum of s with c's sign: one product-and-sum per exponential remains
+        if (a.c < 0.f)
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * a.c;
+            for (int j = 0; j < 32; ++j) r[j] ^= 0x80000000u;
         const uint32_t at = tgt - col, cols = a.n > col ? a.n - col : 0u;
         if (__any_sync(kAll, at < 32u) || cols < 32u) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) if (at == (uint32_t)j || (uint32_t)j >= cols) v[j] = -INFINITY;
+            for (int j = 0; j < 32; ++j) if (at == (uint32_t)j || (uint32_t)j >= cols) r[j] = 0xFF800000u;
         }
-        // four chains each for the maximum and the sum: one would make the warp wait for its own last result 32 times over
-        float m4[4] = {top, v[1], v[2], v[3]}, s4[4] = {0.f, 0.f, 0.f, 0.f};
-        m4[0] = fmaxf(top, v[0]);
+        // several chains for the maximum and the sum: one would make the warp wait for its own last result 32 times over
+        float m4[4];
 #pragma unroll
-        for (int j = 4; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
-        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        for (int j = 0; j < 4; ++j) m4[j] = __uint_as_float(r[j]);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) s4[j & 3] += exp2_fast(v[j] - m);
-        sum = sum * exp2_fast(top - m) + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+        for (int j = 4; j < 28; j += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m4[k] = max3(m4[k], __uint_as_float(r[j + k]), __uint_as_float(r[j + 4 + k]));
+        const float m1 = max3(m4[0], __uint_as_float(r[28]), __uint_as_float(r[29])), m2 = max3(m4[1], __uint_as_float(r[30]), __uint_as_float(r[31]));
+        const float c = fmaxf(fabsf(a.c), 1e-30f);           // a scale of 0: what is left out stays at minus infinity
+        const float m = fmaxf(top, c * fmaxf(max3(m1, m2, m4[2]), m4[3]));
+        const Pair cc = pair(c, c), mm = pair(-m, -m);
+        Pair s[4] = {pair(0.f, 0.f), pair(0.f, 0.f), pair(0.f, 0.f), pair(0.f, 0.f)};
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            const float2 x = split(fma2(pair(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), cc, mm));
+            s[(j >> 1) & 3] = add2(s[(j >> 1) & 3], pair(exp2_fast(x.x), exp2_fast(x.y)));
+        }
+        const float2 f = split(add2(add2(s[0], s[1]), add2(s[2], s[3])));
+        sum = sum * exp2_fast(top - m) + (f.x + f.y);
         top = m;
     }
     __device__ __forceinline__ void finish() {}
@@ -314,27 +342,36 @@ struct GradEpi {
     };
     const Args &a;
     StoreEpi<T> store;
-    uint32_t tgt = 0;
-    float lse2 = 0.f, g = 0.f, at_target = 0.f;
-    __device__ __forceinline__ GradEpi(const Args &args, tile::Staging &staging, const CUtensorMap *out, int lane) : a(args), store(args.out, staging, out, lane) {}
+    uint32_t tgt = 0, next = kNoTarget;
+    float lse2 = 0.f, g = 0.f, at_target = 0.f, grad = 0.f, lse = 0.f, loss = 0.f, factor;
+    __device__ __forceinline__ GradEpi(const Args &args, tile::Staging &staging, const CUtensorMap *out, int lane) : a(args), store(args.out, staging, out, lane) {
+        factor = __ldg(a.factor);
+    }
+    __device__ __forceinline__ void ahead(uint32_t r0) {
+        const uint32_t row = min(r0 + store.lane, a.out.m - 1);      // past the last row: nothing is stored
+        next = __ldg(a.target + row);
+        grad = __ldg(a.grad + row); lse = __ldg(a.lse + row); loss = __ldg(a.loss + row);
+    }
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t n0, uint32_t s, uint32_t p) {
         store.begin(r0, n0, s, p);
-        const uint32_t row = r0 + store.lane;
-        const uint32_t t = row < a.out.m ? __ldg(a.target + row) : kNoTarget;
-        tgt = t - a.col0;
-        g = 0.f; lse2 = 0.f; at_target = 0.f;
-        if (t < a.docs) {
-            g = __ldg(a.grad + row) * __ldg(a.factor);
-            lse2 = __ldg(a.lse + row) * kLog2e;
-            at_target = g * expm1f(-__ldg(a.loss + row));   // -(1 - p) of the target, exact where p is near 1
-        } else tgt = kNoTarget;
+        const bool has = next < a.docs;
+        tgt = has ? next - a.col0 : kNoTarget;
+        g = has ? grad * factor : 0.f;
+        lse2 = has ? lse * kLog2e : 0.f;
+        at_target = has ? g * expm1f(-loss) : 0.f;                  // -(1 - p) of the target, exact where p is near 1
     }
     __device__ __forceinline__ void end() {}
     __device__ __forceinline__ void finish() { store.finish(); }
     __device__ __forceinline__ void chunk(uint32_t (&r)[32], uint32_t col) {
         const bool live = g != 0.f;      // rows without a target may hold anything, NaN included: their G is zero
+        const Pair cc = pair(a.c, a.c), ll = pair(-lse2, -lse2), gg = pair(g, g);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) r[j] = live ? __float_as_uint(g * exp2_fast(fmaf(__uint_as_float(r[j]), a.c, -lse2))) : 0u;
+        for (int j = 0; j < 32; j += 2) {
+            const float2 x = split(fma2(pair(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), cc, ll));
+            const float2 y = split(mul2(gg, pair(exp2_fast(x.x), exp2_fast(x.y))));
+            r[j] = live ? __float_as_uint(y.x) : 0u;
+            r[j + 1] = live ? __float_as_uint(y.y) : 0u;
+        }
         const uint32_t at = tgt - col;
         if (__any_sync(kAll, at < 32u)) {
 #pragma unroll
@@ -816,7 +853,8 @@ static int scores_run(const ap_scaled_rows &a, const ap_scaled_rows &b, uint32_t
     const Operand oa{a.q, a.rows, dim, a.ldq}, ob{b.q, b.rows, dim, b.ldq};
     typename StoreEpi<T>::Args ea{};
     ea.out = out; ea.ld = ldo; ea.m = a.rows; ea.n = b.rows; ea.alpha = alpha; ea.tma = aligned(out, ldo * sizeof(T), 16);
-    const Scales sc{a.scale, b.scale, a.ld_scale, b.ld_scale, a.rows, b.rows,
+    const uint32_t blocks = ceil_div(dim, 128);
+    const Scales sc{a.scale, b.scale, a.scale + (a.rows - 1) * a.ld_scale + blocks, b.scale + (b.rows - 1) * b.ld_scale + blocks, a.ld_scale, b.ld_scale, a.rows, b.rows,
                     aligned(a.scale, a.ld_scale, 4) && aligned(b.scale, b.ld_scale, 4)};
     return run_product<S, StoreEpi<T>>(oa, ob, a.rows, b.rows, dim, pick_n(N, 32, CG, a.rows, b.rows, ceil_div(dim, 128), sms), sc, ea, sms, err, st);
 }

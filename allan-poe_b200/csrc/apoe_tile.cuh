@@ -206,7 +206,6 @@ __device__ __forceinline__ void add_3d(const CUtensorMap *map, const void *src, 
 }
 __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory"); }
-__device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // ---- shared-memory descriptors (version 1) -----------------------------------------------------------------------------
 // K-major, 128-byte swizzle: 8-row groups 1024 bytes apart; a K step of 32 bytes moves the start address
@@ -225,7 +224,7 @@ __device__ __forceinline__ uint64_t desc_sf(uint32_t addr) {
 
 // Scale bytes of the operands (e4m3): [rows][ld], one per 128 values of K.
 struct Scales {
-    const uint8_t *a, *b;
+    const uint8_t *a, *b, *a_end, *b_end;
     size_t lda, ldb;
     uint32_t m, n;
     uint32_t words;            // both: rows on 4-byte boundaries
@@ -238,7 +237,8 @@ struct Staging {
 };
 
 // ---- the kernel --------------------------------------------------------------------------------------------------------
-// Epi: a type with `Args`, `Epi(const Args &, Staging &, const CUtensorMap *out, int lane)`, `begin(first row, first
+// Epi: a type with `Args`, `Epi(const Args &, Staging &, const CUtensorMap *out, int lane)`, `ahead(first row)` as early as
+// possible (what a row needs from global memory is on its way while the tile before is worked on), `begin(first row, first
 // column, split, part)`, `chunk(uint32_t (&r)[32], col)` for 32 columns of the lane's row, `end()` after a tile, `finish()`
 // after the last.  Every lane of a warp makes the same calls.
 // Epi2 other than NoSecond: a second product of the same shape but for an MN-major A, with operands, grid and results of its
@@ -248,6 +248,7 @@ struct Staging {
 struct NoSecond {
     struct Args {};
     __device__ __forceinline__ NoSecond(const Args &, Staging &, const CUtensorMap *, int) {}
+    __device__ __forceinline__ void ahead(uint32_t) {}
     __device__ __forceinline__ void begin(uint32_t, uint32_t, uint32_t, uint32_t) {}
     __device__ __forceinline__ void chunk(uint32_t (&)[32], uint32_t) {}
     __device__ __forceinline__ void end() {}
@@ -427,38 +428,36 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             const uint32_t per_tile = (grid.kblocks + 3) / 4;        // scaled products are never split
             uint32_t t = group, grp = (uint32_t)(warp & 1), sg = grp;   // this warp's next group; its number over all tiles
             auto settle = [&]() { while (t < grid.total && grp >= per_tile) { grp -= per_tile; t += groups; } };
-            auto fetch = [&](uint32_t (&w)[ROWS]) {
+            // The four bytes of a row may start anywhere: the two words around them (none past the last byte) are loaded and
+            // shifted when they are used.  Nothing waits inside, so all rows' loads are under way together.  Rows past the
+            // end read some other row's bytes: their values are zero, their results are not stored.
+            uint32_t lo[ROWS], hi[ROWS], places = 0;
+            auto fetch = [&]() {
                 uint32_t mi, ni, si;
                 locate(grid, t, mi, ni, si);
                 const uint32_t m0 = mi * S::M + rank * 128, n0 = ni * grid.tile_n, kb = grp * 4;
+                places = 0;
 #pragma unroll
                 for (int j = 0; j < ROWS; ++j) {
                     const bool of_a = j < 4;
-                    const uint32_t row = of_a ? m0 + j * 32 + lane : n0 + (j - 4) * 32 + lane, rows = of_a ? scales.m : scales.n;
-                    w[j] = 0x7F7F7F7Fu;                              // rows past the end: 2^0
-                    if (row < rows) {
-                        const uint8_t *p = (of_a ? scales.a + (size_t)row * scales.lda : scales.b + (size_t)row * scales.ldb) + kb;
-                        if (scales.words && (kb + 4 <= grid.kblocks || row + 1 < rows)) w[j] = __ldg(reinterpret_cast<const uint32_t *>(p));
-                        else {                                       // all loads independent: none waits for another
-                            uint32_t v[4];
-#pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i) v[i] = kb + i < grid.kblocks ? __ldg(p + i) : 127u;
-                            w[j] = v[0] | v[1] << 8 | v[2] << 16 | v[3] << 24;
-                        }
-                    }
+                    const uint32_t row = min(of_a ? m0 + j * 32 + lane : n0 + (j - 4) * 32 + lane, (of_a ? scales.m : scales.n) - 1);
+                    const uintptr_t p = (uintptr_t)(of_a ? scales.a + (size_t)row * scales.lda : scales.b + (size_t)row * scales.ldb) + kb;
+                    const uintptr_t last = ((uintptr_t)(of_a ? scales.a_end : scales.b_end) - 1) & ~uintptr_t(3), q = p & ~uintptr_t(3);
+                    places |= ((uint32_t)p & 3u) << (2 * j);
+                    lo[j] = __ldg(reinterpret_cast<const uint32_t *>(q));
+                    hi[j] = scales.words ? 0u : __ldg(reinterpret_cast<const uint32_t *>(q < last ? q + 4 : last));
                 }
             };
-            uint32_t next[ROWS];
             settle();
-            if (t < grid.total) fetch(next);
+            if (t < grid.total) fetch();
             bool ok = true;
             while (t < grid.total) {
                 uint32_t w[12];
 #pragma unroll
-                for (int j = 0; j < 12; ++j) w[j] = j < ROWS ? next[j < ROWS ? j : 0] : 0u;
+                for (int j = 0; j < 12; ++j) w[j] = j < ROWS ? __funnelshift_r(lo[j < ROWS ? j : 0], hi[j < ROWS ? j : 0], 8 * (places >> (2 * j) & 3u)) : 0u;
                 grp += 2;
                 settle();
-                if (t < grid.total) fetch(next);
+                if (t < grid.total) fetch();
                 const uint32_t slot = sg % S::SF_SLOTS;
                 ok = __all_sync(0xFFFFFFFFu, wait(&sempty_bar[slot], ((sg / S::SF_SLOTS) & 1u) ^ 1u, err, 33u));
                 if (!ok) break;
@@ -487,12 +486,17 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         Epi2 epi2(second.epi, staging, out2, lane);
         uint32_t it = 0;
         bool ok = true;
-        auto finish_tile = [&](const Grid &gr, uint32_t t, auto &e) {
-            uint32_t mi, ni, si;
-            locate(gr, t, mi, ni, si);
+        uint32_t mi = 0, ni = 0, si = 0;          // place of the next tile
+        auto look_ahead = [&](uint32_t t) {
+            if (t >= grid.total) return;
+            locate(grid, t, mi, ni, si);
+            epi.ahead(mi * S::M + rank * 128 + quarter * 32);
+        };
+        auto finish_tile = [&](const Grid &gr, auto &e, auto &&then) {
             const int chunks = (int)gr.tile_n / 32, c0 = half ? (chunks + 1) / 2 : 0, c1 = half ? chunks : (chunks + 1) / 2;
             const uint32_t acc = it & 1u, col = ni * gr.tile_n;
             e.begin(mi * S::M + rank * 128 + quarter * 32, col, si, ni * 2 + half);
+            then();
             ok = wait(&tfull_bar[acc], (it >> 1) & 1u, err, 34u);
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) return;
@@ -528,8 +532,11 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             }
             e.end();
         };
-        walk(ok, [&](uint32_t t) { finish_tile(grid, t, epi); ++it; },
-             [&](uint32_t t) { if constexpr (DUAL) { finish_tile(second.grid, t, epi2); ++it; } });
+        look_ahead(group);
+        walk(ok, [&](uint32_t t) { finish_tile(grid, epi, [&] { look_ahead(t + groups); }); ++it; },
+             [&](uint32_t t) {
+                 if constexpr (DUAL) { locate(second.grid, t, mi, ni, si); finish_tile(second.grid, epi2, [] {}); ++it; }
+             });
         epi.finish();
         epi2.finish();
     }
