@@ -457,7 +457,7 @@ _T = None       # torch and what of it the calls below look up each time, set on
 class _Torch:
     def __init__(self):
         import torch
-        self.torch, self.empty = torch, torch.empty
+        self.empty = torch.empty_strided           # the cheapest way to a matrix whose rows are further apart than they are long
         self.f32, self.f16, self.bf16, self.f8, self.u8 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn, torch.uint8
         self.i32, self.u32 = torch.int32, torch.uint32
         self.types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
@@ -513,11 +513,11 @@ def quantize_rows(x, stream=None):
         raise ApoeError(1, "quantize: rows of 0 values")
     device = x.get_device()
     ldq, blocks = (dim + 15) // 16 * 16, (dim + 127) // 128
-    q = x.new_empty((rows, ldq), dtype=T.f8)
-    scale = x.new_empty((rows, blocks), dtype=T.u8)
+    q = T.empty((rows, dim), (ldq, 1), dtype=T.f8, device=x.device)
+    scale = T.empty((rows, blocks), (blocks, 1), dtype=T.u8, device=x.device)
     _check(lib().ap_quantize_rows_device(device, rows, dim, T.types[x.dtype], x.data_ptr(), ld, q.data_ptr(), ldq, scale.data_ptr(), blocks,
                                          T.stream(device) if stream is None else stream))
-    return (q if ldq == dim else q[:, :dim]), scale
+    return q, scale
 
 
 def scaled_scores(a, a_scale, b, b_scale, out_dtype=None, alpha: float = 1.0, out=None, stream=None):
@@ -540,9 +540,7 @@ def scaled_scores(a, a_scale, b, b_scale, out_dtype=None, alpha: float = 1.0, ou
         kind = T.types.get(out_dtype, -1) if out_dtype is not None else TYPE_F32
         unit = 4 if kind == TYPE_F32 else 8                       # values of 16 bytes
         ldo = (n + unit - 1) // unit * unit
-        out = a.new_empty((m, n if m == 1 else ldo), dtype=out_dtype or T.f32)
-        if ldo != n and m != 1:
-            out = out[:, :n]
+        out = T.empty((m, n), (ldo, 1), dtype=out_dtype or T.f32, device=a.device)
     else:
         om, on, ldo = _matrix("out", out, device, T.types)
         if om != m or on != n:
@@ -582,8 +580,9 @@ def softmax_loss_forward(queries, docs, target, scale: float = 1.0, stream=None)
     args = _loss_args(T, queries, docs, target)
     device, rows, n, dim = args[:4]
     size = _workspace_bytes(device, rows, n, dim, 0)
-    ws = queries.new_empty(size, dtype=T.u8)
-    loss, lse = queries.new_empty(rows, dtype=T.f32), queries.new_empty(rows, dtype=T.f32)
+    where = queries.device
+    ws = T.empty((size,), (1,), dtype=T.u8, device=where)
+    loss, lse = T.empty((rows,), (1,), dtype=T.f32, device=where), T.empty((rows,), (1,), dtype=T.f32, device=where)
     _check(lib().ap_softmax_loss_forward_device(*args, scale, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size,
                                                 T.stream(device) if stream is None else stream))
     return loss, lse
@@ -599,12 +598,13 @@ def softmax_loss_backward(queries, docs, target, loss, lse, grad_loss, scale: fl
     pl, pe = _vector("loss", loss, rows, device, f32), _vector("lse", lse, rows, device, f32)
     pg = _vector("grad_loss", grad_loss, rows, device, f32)
     pad = (dim + 7) // 8 * 8
-    gq, gd = queries.new_empty((rows, pad)), queries.new_empty((n, pad))
+    where, kind = queries.device, queries.dtype
+    gq, gd = T.empty((rows, dim), (pad, 1), dtype=kind, device=where), T.empty((n, dim), (pad, 1), dtype=kind, device=where)
     size = _workspace_bytes(device, rows, n, dim, 1)
-    ws = queries.new_empty(size, dtype=T.u8)
+    ws = T.empty((size,), (1,), dtype=T.u8, device=where)
     _check(lib().ap_softmax_loss_backward_device(*args, scale, pl, pe, pg, gq.data_ptr(), pad, gd.data_ptr(), pad, ws.data_ptr(), size,
                                                  T.stream(device) if stream is None else stream))
-    return (gq, gd) if pad == dim else (gq[:, :dim], gd[:, :dim])
+    return gq, gd
 
 
 def dense_check_status(device: int = 0, stream=None) -> None:

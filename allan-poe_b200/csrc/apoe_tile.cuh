@@ -33,7 +33,7 @@ namespace tile {
 
 enum : int { kF16 = 0, kBf16 = 1, kE4m3 = 2 };   // operand kinds
 
-constexpr uint32_t kWaitLimit = 1u << 22;
+constexpr uint32_t kWaitLimit = 1u << 20;         // polls of a few microseconds: seconds, where milliseconds are long
 constexpr int kEpiWarps = 8;                      // two per quarter of the tensor-memory lanes, each half of the columns
 constexpr int kThreads = (kEpiWarps + 4) * 32;    // + TMA producer, MMA issuer, two scale writers (e4m3 only)
 
