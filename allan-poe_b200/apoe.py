@@ -490,10 +490,10 @@ def _matrix(name, t, device, dtypes):
     ld, step = stride
     if step != 1 and cols > 1:
         _bad(name, t, device, dtypes)
+    if rows <= 1:                                   # the stride of a single row means nothing: one that is aligned for every type
+        return rows, cols, (cols + 15) // 16 * 16
     if ld < cols:
-        if rows > 1:
-            _bad(name, t, device, dtypes)
-        ld = cols
+        _bad(name, t, device, dtypes)
     return rows, cols, ld
 
 
@@ -504,7 +504,7 @@ def _vector(name, t, n, device, dtypes):
     return t.data_ptr()
 
 
-def quantize_rows(x, stream=None):
+def quantize_rows(x):
     """Rows in 8 bits: (q float8_e4m3fn [rows, dim], scale uint8 [rows, ceil(dim / 128)]).  The value of q[r, c] is
     q * 2^(scale[r, c // 128] - 127).  x: float32, float16 or bfloat16 matrix.  The rows of q start on 16-byte boundaries."""
     T = _T or _torch()
@@ -516,11 +516,11 @@ def quantize_rows(x, stream=None):
     q = T.empty((rows, dim), (ldq, 1), dtype=T.f8, device=x.device)
     scale = T.empty((rows, blocks), (blocks, 1), dtype=T.u8, device=x.device)
     _check(lib().ap_quantize_rows_device(device, rows, dim, T.types[x.dtype], x.data_ptr(), ld, q.data_ptr(), ldq, scale.data_ptr(), blocks,
-                                         T.stream(device) if stream is None else stream))
+                                         T.stream(device)))
     return q, scale
 
 
-def scaled_scores(a, a_scale, b, b_scale, out_dtype=None, alpha: float = 1.0, out=None, stream=None):
+def scaled_scores(a, a_scale, b, b_scale, out_dtype=None, alpha: float = 1.0, out=None):
     """Scores of 8-bit rows (as `quantize_rows` returns them): [rows of a, rows of b] in out_dtype (float32 by default,
     float16, bfloat16), summed in fp32.  Rows of a and b must start on 16-byte boundaries.  Without `out` the result's rows
     start on 16-byte boundaries too (they are further apart than they are long where a row is no multiple of 16 bytes); any
@@ -552,7 +552,7 @@ def scaled_scores(a, a_scale, b, b_scale, out_dtype=None, alpha: float = 1.0, ou
         raise ApoeError(1, f"scores: {out.dtype}: float32, float16 and bfloat16 are supported")
     _check(lib().ap_scaled_scores_device(device, dim, ScaledRows(m, a.data_ptr(), lda, a_scale.data_ptr(), lsa),
                                          ScaledRows(n, b.data_ptr(), ldb, b_scale.data_ptr(), lsb), alpha, kind, out.data_ptr(), ldo,
-                                         T.stream(device) if stream is None else stream))
+                                         T.stream(device)))
     return out
 
 
@@ -573,7 +573,7 @@ def _workspace_bytes(device, rows, n, dim, backward):
     return size.value
 
 
-def softmax_loss_forward(queries, docs, target, scale: float = 1.0, stream=None):
+def softmax_loss_forward(queries, docs, target, scale: float = 1.0):
     """Softmax loss of queries over all documents without holding the matrix of scores: (loss, lse), float32 [rows].
     queries [rows, dim] and docs [n, dim]: float16 or bfloat16; target: int32 document ids, -1 = the row takes no part."""
     T = _T or _torch()
@@ -584,11 +584,11 @@ def softmax_loss_forward(queries, docs, target, scale: float = 1.0, stream=None)
     ws = T.empty((size,), (1,), dtype=T.u8, device=where)
     loss, lse = T.empty((rows,), (1,), dtype=T.f32, device=where), T.empty((rows,), (1,), dtype=T.f32, device=where)
     _check(lib().ap_softmax_loss_forward_device(*args, scale, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size,
-                                                T.stream(device) if stream is None else stream))
+                                                T.stream(device)))
     return loss, lse
 
 
-def softmax_loss_backward(queries, docs, target, loss, lse, grad_loss, scale: float = 1.0, stream=None):
+def softmax_loss_backward(queries, docs, target, loss, lse, grad_loss, scale: float = 1.0):
     """Gradients of `softmax_loss_forward`: (grad_queries, grad_docs) in the vectors' type.  loss, lse: as the forward call
     returned them; grad_loss: float32 [rows], the gradient of each row's loss (1 / rows for a mean)."""
     T = _T or _torch()
@@ -603,7 +603,7 @@ def softmax_loss_backward(queries, docs, target, loss, lse, grad_loss, scale: fl
     size = _workspace_bytes(device, rows, n, dim, 1)
     ws = T.empty((size,), (1,), dtype=T.u8, device=where)
     _check(lib().ap_softmax_loss_backward_device(*args, scale, pl, pe, pg, gq.data_ptr(), pad, gd.data_ptr(), pad, ws.data_ptr(), size,
-                                                 T.stream(device) if stream is None else stream))
+                                                 T.stream(device)))
     return gq, gd
 
 

@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(256) grad_prep_kernel(const PrepArgs a) {
             for (int i = 1; i < 8; ++i) m = fmaxf(m, s[i]);
             int e = 0;
             if (m > 0.f && m < INFINITY) frexpf(m, &e);            // m <= 2^e
-            const int k = min(max(14 - e, -100), 100);
+            const int k = min(max(14 - e, -126), 126);
             a.factor[0] = ldexpf(1.f, k);
             a.factor[1] = ldexpf(a.scale, -k);
         }
@@ -596,22 +596,23 @@ static int launch(void (*kernel)(Args), uint32_t grid, const Args &args, cudaStr
     return AP_OK;
 }
 
-// What a tile costs, in K blocks of a full tile (about 0.5 us on a pair of SMs): its K blocks, each in proportion to its columns
-// and its rows' share of the loads but never below 0.6 of a full one, and 1.5 for its ends; a short K leaves the epilogue
-// (2.5 us for 256 columns) to wait for.  Measured on pairs at K = 2048, us per K block: 16 bits 0.34 / 0.41 / 0.51 at 128 / 192 /
-// 256 columns, 8 bits 0.36 / 0.39 / 0.48 / 0.53 at 32 to 96 / 128 / 192 / 224.
-static double tile_cost(uint32_t tile_n, uint32_t kblocks) {
-    return std::max(kblocks * std::max((tile_n + 128) / 384.0, 0.6) + 1.5, 5.0 * tile_n / 256.0 + 1.0);
+// What a tile costs, in K blocks of a full 16-bit tile (0.39 us on a pair of SMs): its K blocks, whose cost falls more slowly
+// than their columns, and 1.5 for its ends; a short K leaves the epilogue (2 us for 256 columns) to wait for.  Measured on
+// pairs at K = 4096, us per K block: 16 bits 0.26 / 0.29 / 0.35 / 0.39 at 64 / 128 / 224 / 256 columns, 8 bits 0.34 / 0.36 / 0.40
+// at 64 / 128 / 224.
+static double tile_cost(uint32_t tile_n, uint32_t kblocks, bool scaled = false) {
+    const double block = scaled ? (tile_n + 900) / 1100.0 : std::max((tile_n + 192) / 448.0, 0.66);
+    return std::max(kblocks * block + 1.5, 5.0 * tile_n / 256.0 + 1.0);
 }
 // Columns of a tile: as many as the shape allows, unless narrower tiles fill the rounds of the persistent grid better
 // (1000 x 10007 x 1024: 160 tiles of 256 x 256 on 74 pairs take three rounds, 212 of 256 x 192 three shorter ones).
-static uint32_t pick_n(uint32_t most, uint32_t least, int cg, uint32_t m, uint32_t n, uint32_t kblocks, int sms) {
+static uint32_t pick_n(uint32_t most, uint32_t least, int cg, uint32_t m, uint32_t n, uint32_t kblocks, int sms, bool scaled = false) {
     const uint32_t groups = (uint32_t)std::max(1, sms / cg), tiles_m = ceil_div(m, 128 * (uint32_t)cg);
     uint32_t best = most;
     double best_cost = 1e300;
     for (uint32_t w = most; w >= least; w -= 32) {
-        const double cost = (double)(((uint64_t)tiles_m * ceil_div(n, w) + groups - 1) / groups) * tile_cost(w, kblocks);
-        if (cost < best_cost * 0.97) { best_cost = cost; best = w; }
+        const double cost = (double)(((uint64_t)tiles_m * ceil_div(n, w) + groups - 1) / groups) * tile_cost(w, kblocks, scaled);
+        if (cost < best_cost * 0.985) { best_cost = cost; best = w; }
     }
     return best;
 }
@@ -738,8 +739,8 @@ static Cut pick_cut(uint32_t rows, uint32_t docs, uint32_t dim, uint32_t most_sp
     for (uint32_t s = 1; s <= most_splits && (s == 1 || kx / s >= 8); ++s) {
         if (ceil_div(kx, ceil_div(kx, s)) != s) continue;
         const Cut c{s, best.n};
-        // a part is a matrix of fp32 sums that is written and read once more: its time at 6.5 TB/s, in units of 0.5 us
-        const double cost = deal_of(rows, docs, dim, c, sms).cost + (s > 1 ? 2.0 + s * (double)rows * dim * 6.0 / 6.5e12 / 0.5e-6 : 0.0);
+        // a part is a matrix of fp32 sums that is written and read once more: its time at 6.5 TB/s, in units of 0.39 us
+        const double cost = deal_of(rows, docs, dim, c, sms).cost + (s > 1 ? 2.0 + s * (double)rows * dim * 6.0 / 6.5e12 / 0.39e-6 : 0.0);
         if (cost < best_cost * 0.98) { best_cost = cost; best.splits = s; }
     }
     return best;
@@ -856,7 +857,7 @@ static int scores_run(const ap_scaled_rows &a, const ap_scaled_rows &b, uint32_t
     const uint32_t blocks = ceil_div(dim, 128);
     const Scales sc{a.scale, b.scale, a.scale + (a.rows - 1) * a.ld_scale + blocks, b.scale + (b.rows - 1) * b.ld_scale + blocks, a.ld_scale, b.ld_scale, a.rows, b.rows,
                     aligned(a.scale, a.ld_scale, 4) && aligned(b.scale, b.ld_scale, 4)};
-    return run_product<S, StoreEpi<T>>(oa, ob, a.rows, b.rows, dim, pick_n(N, 32, CG, a.rows, b.rows, ceil_div(dim, 128), sms), sc, ea, sms, err, st);
+    return run_product<S, StoreEpi<T>>(oa, ob, a.rows, b.rows, dim, pick_n(N, 32, CG, a.rows, b.rows, ceil_div(dim, 128), sms, true), sc, ea, sms, err, st);
 }
 template <class T>
 static int scores_pick(const ap_scaled_rows &a, const ap_scaled_rows &b, uint32_t dim, float alpha, void *out, uint64_t ldo, int sms, uint32_t *err,
@@ -942,7 +943,7 @@ extern "C" int ap_scaled_scores_device(int device, uint32_t dim, const ap_scaled
         return fail(AP_ERR_ARG, "scores: a row stride is shorter than a row");
     if (!aligned(a->q, a->ldq, 16) || !aligned(b->q, b->ldq, 16)) return fail(AP_ERR_ARG, "scores: 8-bit rows start on 16-byte boundaries (base and stride)");
     if ((uintptr_t)out % (uint32_t)size) return fail(AP_ERR_ARG, "scores: the output is not aligned to its type");
-    if ((uint64_t)ceil_div(a->rows, 128) * ceil_div(b->rows, 64) >= (1ull << 32)) return fail(AP_ERR_LIMIT, "scores: %u x %u scores in one call", a->rows, b->rows);
+    if ((uint64_t)ceil_div(a->rows, 128) * ceil_div(b->rows, 32) >= (1ull << 31)) return fail(AP_ERR_LIMIT, "scores: %u x %u scores in one call", a->rows, b->rows);
     DeviceScope scope;
     AP_TRY(scope.enter(device));
     int sms;
@@ -957,6 +958,8 @@ extern "C" int ap_scaled_scores_device(int device, uint32_t dim, const ap_scaled
 extern "C" int ap_softmax_loss_workspace(int device, uint32_t rows, uint32_t docs, uint32_t dim, int backward, size_t *bytes) {
     if (!bytes) return fail(AP_ERR_ARG, "softmax loss: null argument");
     if (rows == 0 || docs == 0 || dim == 0) return fail(AP_ERR_ARG, "softmax loss: %u queries, %u documents, %u values: none may be 0", rows, docs, dim);
+    if (rows > (1u << 20) || docs > (1u << 30) || dim > (1u << 16))
+        return fail(AP_ERR_LIMIT, "softmax loss: up to 2^20 queries, 2^30 documents, 2^16 values");
     if (!backward) { *bytes = forward_plan(rows, docs).bytes; return AP_OK; }
     int sms;
     AP_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));

@@ -34,6 +34,7 @@ namespace tile {
 enum : int { kF16 = 0, kBf16 = 1, kE4m3 = 2 };   // operand kinds
 
 constexpr uint32_t kWaitLimit = 1u << 20;         // polls of a few microseconds: seconds, where milliseconds are long
+constexpr uint32_t kWarp = 0xFFFFFFFFu;
 constexpr int kEpiWarps = 8;                      // two per quarter of the tensor-memory lanes, each half of the columns
 constexpr int kThreads = (kEpiWarps + 4) * 32;    // + TMA producer, MMA issuer, two scale writers (e4m3 only)
 
@@ -124,6 +125,23 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, uint32_t *e
     if (err) atomicExch(err, code);
     return false;
 }
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {   // one answer for the warp
+    return __all_sync(kWarp, wait(bar, parity, err, code));
+}
+__device__ __forceinline__ bool ask(uint64_t *bar, uint32_t parity) {      // without waiting
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool ask_cluster(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
     for (uint32_t i = 0; i < kWaitLimit; ++i) {
         uint32_t ok;
@@ -209,7 +227,7 @@ template <int LEFT> __device__ __forceinline__ void store_wait_read() { asm vola
 
 // ---- shared-memory descriptors (version 1) -----------------------------------------------------------------------------
 // K-major, 128-byte swizzle: 8-row groups 1024 bytes apart; a K step of 32 bytes moves the start address
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+__host__ __device__ constexpr uint64_t desc_k(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 // MN-major, 128-byte swizzle: slabs of 64 M (N) values x 64 K rows of 128 bytes, 8192 bytes apart (bits 16-29); groups of 8
@@ -217,6 +235,7 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
 __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
+__device__ __forceinline__ uint64_t desc_of(uint32_t hi, uint32_t lo) { return (uint64_t)hi << 32 | lo; }
 // scale words: no swizzle, 8-row groups of 16-byte rows 128 bytes apart
 __device__ __forceinline__ uint64_t desc_sf(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
@@ -324,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         // As in the MMA warp, all lanes walk the loop and one elected lane issues: with the loop inside a one-lane branch the
         // products were issued at 215 cycles each (e4m3, 112 needed) and 170 (f16, 128 needed).
         uint32_t s = 0, phase = 0, issued = 0;
-        bool ok = true;
+        bool ok = true, free = true;
         auto load = [&](const CUtensorMap &ma, const CUtensorMap &mb, const Grid &gr, uint32_t t, auto amn) {
             constexpr bool AMN = decltype(amn)::value;
             const uint32_t br = gr.tile_n / CG, bytes = (S::A_BYTES + (S::BMN ? (br + 63) / 64 * 8192 : br * 128)) * CG;
@@ -333,13 +352,19 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             const int m0 = (int)(mi * S::M + rank * 128), n0 = (int)(ni * gr.tile_n + rank * br);
             const uint32_t k0 = si * gr.kper, k1 = min(k0 + gr.kper, gr.kblocks);
             for (uint32_t kb = k0; kb < k1; ++kb) {
-                ok = wait(&empty_bar[s], phase ^ 1u, err, 30u);
-                if (!ok) break;
+                if (!free) {
+                    ok = wait_warp(&empty_bar[s], phase ^ 1u, err, 30u);
+                    if (!ok) break;
+                }
                 uint8_t *st = smem + s * S::STAGE_BYTES;
-                const uint32_t bar = CG == 2 ? leader_addr(&full_bar[s]) : smem_u32(&full_bar[s]);
+                uint64_t *full = &full_bar[s];
+                const uint32_t bar = CG == 2 ? leader_addr(full) : smem_u32(full);
                 const int k = (int)(kb * S::K);
+                ++issued;
+                if (++s == S::STAGES) { s = 0; phase ^= 1u; }
+                const bool asked = ask(&empty_bar[s], phase ^ 1u);   // the next stage's, while this one's loads are issued
                 if (elect_one()) {
-                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], bytes);
+                    if (rank == 0) mbar_arrive_expect_tx(full, bytes);
                     if (AMN) {
                         load_2d<CG>(st, &ma, m0, k, bar);
                         load_2d<CG>(st + 8192, &ma, m0 + 64, k, bar);
@@ -348,9 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                         for (uint32_t j = 0; j * 64 < br; ++j) load_2d<CG>(st + S::A_BYTES + j * 8192, &mb, n0 + (int)j * 64, k, bar);
                     else load_2d<CG>(st + S::A_BYTES, &mb, k, n0, bar);
                 }
-                __syncwarp();
-                ++issued;
-                if (++s == S::STAGES) { s = 0; phase ^= 1u; }
+                free = __all_sync(kWarp, asked);                     // one answer for the warp
             }
         };
         walk(ok, [&](uint32_t t) { load(map_a, map_b, grid, t, std::integral_constant<bool, S::AMN>{}); },
@@ -361,32 +384,49 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     } else if (warp == kEpiWarps + 1) {
         // ---------------- MMA issue (the leader; the warp walks the loop together and one elected lane issues) -----------
         if (rank == 0) {
+            // A wait on a barrier that is ready costs about 145 cycles from issue to use, the products of a K block 256 to 512:
+            // the next stage's barrier is asked while this one's products are issued, and only the low words of the
+            // descriptors change.
+            constexpr uint32_t A_STEP = 2, B_STEP = S::BMN ? 128 : 2;             // a K step, in the address field's 16 bytes
+            constexpr uint32_t DESC_HI = (uint32_t)(desc_k(0) >> 32);             // the same for all kinds
+            constexpr uint32_t LBO_K = 1u << 16, LBO_MN = (8192u >> 4) << 16;
+            const uint32_t base = (smem_u32(smem) & 0x3FFFFu) >> 4;
             uint32_t s = 0, phase = 0, it = 0, sg = 0, sf = 0;
-            bool ok = true;
+            bool ok = true, ready = false, sready = false;
             auto multiply = [&](const Grid &gr, uint32_t t, auto amn) {
                 constexpr bool AMN = decltype(amn)::value;
                 constexpr uint32_t FLAG = AMN && !S::AMN ? 1u << 15 : 0u;
                 const uint32_t si = gr.kper < gr.kblocks ? t / (gr.tiles_m * gr.tiles_n) : 0u;
                 const uint32_t k0 = si * gr.kper, k1 = min(k0 + gr.kper, gr.kblocks);
                 const uint32_t acc = it & 1u, d = tmem + acc * S::N;
-                ok = wait(&tempty_bar[acc], ((it >> 1) & 1u) ^ 1u, err, 31u);
+                uint32_t idesc = S::IDESC | ((gr.tile_n >> 3) << 17) | FLAG, add = 0;
+                ok = wait_warp(&tempty_bar[acc], ((it >> 1) & 1u) ^ 1u, err, 31u);
                 if (!ok) return;
                 fence_after();
                 for (uint32_t kb = k0; kb < k1; ++kb) {
-                    ok = wait(&full_bar[s], phase, err, 32u);
-                    if (!ok) break;
+                    if (!ready) {
+                        ok = wait_warp(&full_bar[s], phase, err, 32u);
+                        if (!ok) break;
+                    }
                     const uint32_t slot = sg % (S::SCALED ? S::SF_SLOTS : 1);
-                    const bool fresh = S::SCALED && kb % 4 == 0;
+                    const bool fresh = S::SCALED && kb % 4 == 0, last = kb + 1 == k1;
                     if (fresh) {
                         // the slot's own scale columns: the products that read them last have completed (their commit freed it)
-                        ok = wait_cluster(&sfull_bar[slot], (sg / (S::SCALED ? S::SF_SLOTS : 1)) & 1u, err, 35u);
-                        if (!ok) break;
+                        if (!sready) {
+                            ok = __all_sync(kWarp, wait_cluster(&sfull_bar[slot], (sg / (S::SCALED ? S::SF_SLOTS : 1)) & 1u, err, 35u));
+                            if (!ok) break;
+                        }
                         sf = tmem + 2 * S::N + slot * 12;
                     }
                     fence_after();
-                    const uint32_t a = smem_u32(smem) + s * S::STAGE_BYTES, b = a + S::A_BYTES;
-                    const uint64_t da = AMN ? desc_mn(a) : desc_k(a), db = S::BMN ? desc_mn(b) : desc_k(b);
-                    const uint32_t idesc = (S::SCALED ? S::IDESC | ((kb & 3u) << 4) | ((kb & 3u) << 29) : S::IDESC) | ((gr.tile_n >> 3) << 17) | FLAG;
+                    const uint32_t here = s, a = base + s * (S::STAGE_BYTES >> 4), b = a + (S::A_BYTES >> 4);
+                    if (++s == S::STAGES) { s = 0; phase ^= 1u; }
+                    bool sasked = false;
+                    const bool asked = ask(&full_bar[s], phase);   // the next stage's (after the last one: of the next tile)
+                    if (S::SCALED && (kb % 4 == 3 || last)) {
+                        ++sg;
+                        sasked = ask_cluster(&sfull_bar[sg % (S::SCALED ? S::SF_SLOTS : 1)], (sg / (S::SCALED ? S::SF_SLOTS : 1)) & 1u);
+                    }
                     if (elect_one()) {
                         if (fresh) {
                             const uint32_t w = smem_u32(smem) + S::STAGES * S::STAGE_BYTES + slot * S::SF_BYTES;
@@ -395,19 +435,19 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                             if (S::N > 128) copy_scales<CG>(sf + 8, desc_sf(w + 1024));
                         }
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {             // the address field counts 16 bytes: 32 or 2048 bytes a step
-                            const uint64_t ia = da + kk * (AMN ? 128 : 2), ib = db + kk * (S::BMN ? 128 : 2);
-                            const uint32_t add = (kb != k0 || kk != 0) ? 1u : 0u;
-                            if (S::SCALED) mma_mx8<CG>(d, ia, ib, idesc, sf, sf + 4, add);
-                            else mma_f16<CG>(d, ia, ib, idesc, add);
+                        for (int kk = 0; kk < 4; ++kk) {
+                            const uint64_t da = desc_of(DESC_HI, (a + kk * (AMN ? 128 : A_STEP)) | (AMN ? LBO_MN : LBO_K));
+                            const uint64_t db = desc_of(DESC_HI, (b + kk * B_STEP) | (S::BMN ? LBO_MN : LBO_K));
+                            if (S::SCALED) mma_mx8<CG>(d, da, db, idesc | ((kb & 3u) << 4) | ((kb & 3u) << 29), sf, sf + 4, add | kk);
+                            else mma_f16<CG>(d, da, db, idesc, add | kk);
                         }
-                        commit<CG>(&empty_bar[s]);
-                        if (S::SCALED && (kb % 4 == 3 || kb + 1 == k1)) commit<CG>(&sempty_bar[slot]);
-                        if (kb + 1 == k1) commit<CG>(&tfull_bar[acc]);
+                        commit<CG>(&empty_bar[here]);
+                        if (S::SCALED && (kb % 4 == 3 || last)) commit<CG>(&sempty_bar[slot]);
+                        if (last) commit<CG>(&tfull_bar[acc]);
                     }
-                    __syncwarp();
-                    if (S::SCALED && (kb % 4 == 3 || kb + 1 == k1)) ++sg;
-                    if (++s == S::STAGES) { s = 0; phase ^= 1u; }
+                    add = 1;
+                    ready = __all_sync(kWarp, asked);          // one answer for the warp
+                    if (S::SCALED && (kb % 4 == 3 || last)) sready = __all_sync(kWarp, sasked);
                 }
             };
             walk(ok, [&](uint32_t t) { multiply(grid, t, std::integral_constant<bool, S::AMN>{}); ++it; },
@@ -459,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 settle();
                 if (t < grid.total) fetch();
                 const uint32_t slot = sg % S::SF_SLOTS;
-                ok = __all_sync(0xFFFFFFFFu, wait(&sempty_bar[slot], ((sg / S::SF_SLOTS) & 1u) ^ 1u, err, 33u));
+                ok = wait_warp(&sempty_bar[slot], ((sg / S::SF_SLOTS) & 1u) ^ 1u, err, 33u);
                 if (!ok) break;
                 // lane l of the 32 keeps rows l, l + 32, l + 64, l + 96 in its 16 bytes
                 uint4 *dst = reinterpret_cast<uint4 *>(smem + S::STAGES * S::STAGE_BYTES + slot * S::SF_BYTES);
@@ -497,8 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             const uint32_t acc = it & 1u, col = ni * gr.tile_n;
             e.begin(mi * S::M + rank * 128 + quarter * 32, col, si, ni * 2 + half);
             then();
-            ok = wait(&tfull_bar[acc], (it >> 1) & 1u, err, 34u);
-            ok = __all_sync(0xFFFFFFFFu, ok);
+            ok = wait_warp(&tfull_bar[acc], (it >> 1) & 1u, err, 34u);
             if (!ok) return;
             fence_after();
             const uint32_t src = tmem + ((uint32_t)(32 * quarter) << 16) + acc * S::N;

@@ -368,6 +368,38 @@ def test_loss_ignores_what_lies_behind_a_row(rows, docs, dim, dtype):
         assert bool((gq[:, dim:] == 3.0).all()) and bool((gd[:, dim:] == 3.0).all())
 
 
+def test_gradients_scale_with_the_losses_gradient():
+    """Times a power of two the same bits (bf16 has f32's range); extreme sizes of it neither overflow nor vanish on the way."""
+    q, d, t, scale = loss_case(140, 400, 64, torch.bfloat16, 17)
+    grad = torch.rand(140, generator=gen(18), device=DEV) + 0.5
+    loss, lse = apoe.softmax_loss_forward(q, d, t, scale)
+    dq, dd = apoe.softmax_loss_backward(q, d, t, loss, lse, grad, scale)
+    for k in (-90, -20, 3, 100):
+        gq, gd = apoe.softmax_loss_backward(q, d, t, loss, lse, grad * 2.0 ** k, scale)
+        assert torch.equal(gq.double(), dq.double() * 2.0 ** k) and torch.equal(gd.double(), dd.double() * 2.0 ** k)
+    gq, gd = apoe.softmax_loss_backward(q, d, t, loss, lse, torch.zeros_like(grad), scale)
+    assert not gq.any() and not gd.any()
+    h, e = q.half(), d.half()
+    loss, lse = apoe.softmax_loss_forward(h, e, t, scale)
+    big = grad * 2e38                                     # below 3e38
+    gq, _ = apoe.softmax_loss_backward(h, e, t, loss, lse, big, 1e-36)     # f16 results of ordinary size from gradients near 3e38
+    assert bool(torch.isfinite(gq).all()) and bool((gq[t >= 0] != 0).any())
+
+
+def test_single_rows_of_any_length():
+    g = gen(19)
+    for dim in (1, 7, 100, 333):
+        x = torch.randn(1, dim, generator=g, device=DEV)
+        q, s = apoe.quantize_rows(x)
+        check_scores(apoe.scaled_scores(q, s, q, s), q, s, q, s)
+        h = x.half()
+        t = torch.zeros(1, dtype=torch.int32, device=DEV)
+        loss, lse = apoe.softmax_loss_forward(h, h, t, 0.5)
+        assert float(loss) == 0.0 and abs(float(lse) - 0.5 * float((h.double() ** 2).sum())) < 1e-4 * float((h.double() ** 2).sum())
+        dq, dd = apoe.softmax_loss_backward(h, h, t, loss, lse, torch.ones(1, device=DEV), 0.5)
+        assert not dq.any() and not dd.any()
+
+
 def test_targets_out_of_range_show_and_give_no_gradient():
     q, d, t, scale = loss_case(40, 300, 64, torch.float16, 12, pad=False)
     grad = torch.full((40,), 0.1, device=DEV)
