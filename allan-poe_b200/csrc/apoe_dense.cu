@@ -247,6 +247,7 @@ struct StoreEpi {
                     const T v = *reinterpret_cast<const T *>(box + row * 64 + (((k / PER) ^ ((row >> 1) & 3)) << 4) + (k % PER) * sizeof(T));
                     if (in && row < rows) o[(size_t)row * a.ld] = v;
                 }
+                if (lane == 0) tile::store_commit();       // an empty group: the wait above counts one group per box
                 __syncwarp();
             }
         }

@@ -454,6 +454,32 @@ def test_pieces_of_the_documents_join(rows, docs):
     check_grads(q, d, t, scale, grad, loss, lse, dq, dd)
 
 
+@pytest.mark.parametrize("rows,docs,dim", [(12, 71344, 144), (4, 55990, 200), (150, 60000, 72), (40, 30000, 328)])
+def test_ragged_columns_over_many_tiles(rows, docs, dim):
+    """Many tiles per SM whose last columns are written element by element while the others' copies are still on their way:
+    every document's gradient, several times over, and the same bits each time."""
+    q, d, t, scale = loss_case(rows, docs, dim, torch.bfloat16, 71)
+    grad = torch.full((rows,), 1.0 / rows, device=DEV)
+    loss, lse = apoe.softmax_loss_forward(q, d, t, scale)
+    first = apoe.softmax_loss_backward(q, d, t, loss, lse, grad, scale)
+    check_grads(q, d, t, scale, grad, loss, lse, *first)
+    for _ in range(8):
+        again = apoe.softmax_loss_backward(q, d, t, loss, lse, grad, scale)
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(30000, 200), (60000, 45), (20000, 233)])
+def test_ragged_scores_over_many_tiles(m, n, dtype):
+    g = gen(72)
+    qa, sa = apoe.quantize_rows(torch.randn(m, 64, generator=g, device=DEV))
+    qb, sb = apoe.quantize_rows(torch.randn(n, 64, generator=g, device=DEV))
+    first = apoe.scaled_scores(qa, sa, qb, sb, out_dtype=dtype)
+    check_scores(first, qa, sa, qb, sb)
+    for _ in range(8):
+        assert torch.equal(apoe.scaled_scores(qa, sa, qb, sb, out_dtype=dtype), first)
+
+
 def test_same_call_same_bits_on_any_stream():
     q, d, t, scale = loss_case(700, 3000, 256, torch.bfloat16, 31)
     grad = torch.full((700,), 1 / 700, device=DEV)
