@@ -274,7 +274,7 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) { Pair d; asm("add.rn.f32x2
 __device__ __forceinline__ Pair mul2(Pair a, Pair b) { Pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
 
 // Running maximum and sum of 2^(l log2 e) of a row over the columns of a tile, the target's column left out: the target's
-// own logit is computed on its own, in fp32 over all of K, because the loss is a difference against it.
+// own logit is computed apart and more exactly, because the loss is a difference against it.
 struct LseEpi {
     struct Args {
         float2 *part;            // [rows][parts]: maximum and sum, in base 2
@@ -393,7 +393,7 @@ struct JoinArgs {
     const uint32_t *target;
     float *loss, *lse;
     uint32_t rows, docs, dim, parts, first, last;
-    float scale;
+    float scale, c;              // c: what the tiles took the products times
 };
 // One warp per row.  With z = log(sum of the others) - (target's logit): loss = log(1 + e^z), which keeps its digits where the
 // row is nearly certain (z << 0) and where it is hopeless; lse = target's logit + loss.
@@ -429,25 +429,28 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs a) {
     float loss = 0.f, lse = 0.f;
     if (t < a.docs) {
         const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx, *w = static_cast<const T *>(a.w) + (size_t)t * a.ldw;
-        float d0 = 0.f, d1 = 0.f;
+        // products of 16-bit values are exact; eight of them are summed in fp32, the sums in 64 bits
+        double dot = 0.0;
         uint32_t i = lane * 8;
         for (; i + 8 <= a.dim; i += 256) {
             const uint4 u = __ldg(reinterpret_cast<const uint4 *>(x + i)), v = __ldg(reinterpret_cast<const uint4 *>(w + i));
             const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
+            float d0 = 0.f, d1 = 0.f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float2 fu = Half16<T>::unpack(us[k]), fv = Half16<T>::unpack(vs[k]);
                 d0 = fmaf(fu.x, fv.x, d0); d1 = fmaf(fu.y, fv.y, d1);
             }
+            dot += (double)(d0 + d1);
         }
-        for (; i < a.dim; ++i) { d0 = fmaf(load_as_float(x + i), load_as_float(w + i), d0); if ((i & 7) == 7) break; }
-        float dot = d0 + d1;
+        for (uint32_t k = i; k < min(i + 8, a.dim); ++k) dot += (double)(load_as_float(x + k) * load_as_float(w + k));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(kAll, dot, o);
-        const float at = a.scale * dot;
-        const float z = (log2f(sum) + top) * kLn2 - at;           // sum = 0 (one document): minus infinity, loss 0
+        // the logits were taken times c, a rounding of scale * log2 e: the maximum is put right, the sum holds differences only
+        const double at = (double)a.scale * dot, exact = (double)a.scale * 1.4426950408889634 / (double)a.c;
+        const float z = (float)(((double)top * (a.c != 0.f ? exact : 1.0) + log2((double)sum)) * 0.6931471805599453 - at);   // sum = 0 (one document): minus infinity, loss 0
         loss = z > 0.f ? z + log1pf(expf(-z)) : log1pf(expf(z));  // a NaN stays one
-        lse = at + loss;
+        lse = (float)(at + (double)loss);
     } else if (t != kNoTarget) loss = lse = __int_as_float(0x7FFFFFFF);
     if (lane == 0) { a.loss[row] = loss; a.lse[row] = lse; }
 }
@@ -789,7 +792,7 @@ static int forward_run(const LossCall &c, const ForwardPlan &p, uint8_t *ws, flo
         LseEpi::Args ea{part, c.target, 2 * ceil_div(n, tn), c.rows, n, v0, c.scale * kLog2e};
         AP_TRY((run_product<S, LseEpi>(x, w, c.rows, n, c.dim, tn, Scales{}, ea, c.sms, c.err, c.st)));
         JoinArgs ja{part, carry, c.x, c.w, c.ldx, c.ldw, c.target, loss, lse, c.rows, c.docs, c.dim, ea.parts, v0 == 0 ? 1u : 0u,
-                    v0 + n == c.docs ? 1u : 0u, c.scale};
+                    v0 + n == c.docs ? 1u : 0u, c.scale, ea.c};
         AP_TRY(launch(loss_join_kernel<T>, ceil_div(c.rows, 8), ja, c.st));
     }
     return AP_OK;
