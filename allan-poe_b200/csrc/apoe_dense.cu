@@ -22,7 +22,7 @@ using tile::Grid;
 using tile::Scales;
 
 constexpr uint32_t kNoTarget = 0xFFFFFFFFu;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 
 __device__ uint32_t dense_error_word;   // raised by a kernel whose bounded wait ran out; read by ap_dense_check_status
@@ -99,8 +99,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantArgs a) {
     constexpr uint32_t STEP = kQuantUnroll * PER;
     const uint32_t lane = threadIdx.x & 31, sub = lane / LANES, c0 = (lane % LANES) * V;
     const uint32_t warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    tile::pdl_launch();
     tile::pdl_wait();
+    tile::pdl_launch();
     const uint32_t it0 = warp * STEP + sub;
     uint32_t row[kQuantUnroll], c[kQuantUnroll];      // first value of the lane: row, and place in it (kFlat: block, 0)
     uint4 raw[kQuantUnroll];
@@ -399,14 +399,35 @@ struct JoinArgs {
 // row is nearly certain (z << 0) and where it is hopeless; lse = target's logit + loss.
 template <class T>
 __global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs a) {
-    tile::pdl_launch();
-    tile::pdl_wait();
     const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const uint32_t t = a.last && row < a.rows ? a.target[row] : kNoTarget;
+    double dot = 0.0;                    // the target's logit, from inputs that are complete: while the tiles are still at work
+    if (t < a.docs) {
+        // products of 16-bit values are exact; eight of them are summed in fp32, the sums in 64 bits
+        const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx, *w = static_cast<const T *>(a.w) + (size_t)t * a.ldw;
+        uint32_t i = lane * 8;
+        for (; i + 8 <= a.dim; i += 256) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(x + i)), v = __ldg(reinterpret_cast<const uint4 *>(w + i));
+            const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
+            float d0 = 0.f, d1 = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 fu = Half16<T>::unpack(us[k]), fv = Half16<T>::unpack(vs[k]);
+                d0 = fmaf(fu.x, fv.x, d0); d1 = fmaf(fu.y, fv.y, d1);
+            }
+            dot += (double)(d0 + d1);
+        }
+        for (uint32_t k = i; k < min(i + 8, a.dim); ++k) dot += (double)(load_as_float(x + k) * load_as_float(w + k));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(kAll, dot, o);
+    }
+    tile::pdl_wait();
+    tile::pdl_launch();
     if (row >= a.rows) return;
     float top = -1.0e30f, sum = 0.f;
     const float2 *p = a.part + (size_t)row * a.parts;
     for (uint32_t i = lane; i < a.parts; i += 32) {
-        const float2 e = __ldg(p + i);
+        const float2 e = p[i];
         const float m = fmaxf(top, e.x);
         sum = sum * exp2f(top - m) + e.y * exp2f(e.x - m);
         top = m;
@@ -425,30 +446,11 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs a) {
         top = m;
     }
     if (!a.last) { if (lane == 0) a.carry[row] = make_float2(top, sum); return; }
-    const uint32_t t = a.target[row];
     float loss = 0.f, lse = 0.f;
     if (t < a.docs) {
-        const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx, *w = static_cast<const T *>(a.w) + (size_t)t * a.ldw;
-        // products of 16-bit values are exact; eight of them are summed in fp32, the sums in 64 bits
-        double dot = 0.0;
-        uint32_t i = lane * 8;
-        for (; i + 8 <= a.dim; i += 256) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(x + i)), v = __ldg(reinterpret_cast<const uint4 *>(w + i));
-            const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
-            float d0 = 0.f, d1 = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 fu = Half16<T>::unpack(us[k]), fv = Half16<T>::unpack(vs[k]);
-                d0 = fmaf(fu.x, fv.x, d0); d1 = fmaf(fu.y, fv.y, d1);
-            }
-            dot += (double)(d0 + d1);
-        }
-        for (uint32_t k = i; k < min(i + 8, a.dim); ++k) dot += (double)(load_as_float(x + k) * load_as_float(w + k));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(kAll, dot, o);
         // the logits were taken times c, a rounding of scale * log2 e: the maximum is put right, the sum holds differences only
-        const double at = (double)a.scale * dot, exact = (double)a.scale * 1.4426950408889634 / (double)a.c;
-        const float z = (float)(((double)top * (a.c != 0.f ? exact : 1.0) + log2((double)sum)) * 0.6931471805599453 - at);   // sum = 0 (one document): minus infinity, loss 0
+        const double at = (double)a.scale * dot, exact = a.c != 0.f ? (double)a.scale * 1.4426950408889634 / (double)a.c : 1.0;
+        const float z = (float)(((double)top * exact + log2((double)sum)) * 0.6931471805599453 - at);   // one document: minus infinity, loss 0
         loss = z > 0.f ? z + log1pf(expf(-z)) : log1pf(expf(z));  // a NaN stays one
         lse = (float)(at + (double)loss);
     } else if (t != kNoTarget) loss = lse = __int_as_float(0x7FFFFFFF);
@@ -469,8 +471,8 @@ struct PrepArgs {
 // inside a product); block 0 also finds the factor of G from the largest |grad| of the rows that count.
 template <class T>
 __global__ void __launch_bounds__(256) grad_prep_kernel(const PrepArgs a) {
-    tile::pdl_launch();
     tile::pdl_wait();
+    tile::pdl_launch();
     if (blockIdx.x == 0) {
         __shared__ float s[8];
         float m = 0.f;
@@ -511,8 +513,8 @@ struct FinishArgs {
 // dX from the partial sums of the splits (added in a fixed order), rounded once
 template <class T>
 __global__ void __launch_bounds__(256) grad_finish_kernel(const FinishArgs a) {
-    tile::pdl_launch();
     tile::pdl_wait();
+    tile::pdl_launch();
     const float f = a.factor[1];
     const uint32_t quads = (a.dim + 3) / 4;
     const uint64_t total = (uint64_t)a.rows * quads;
@@ -673,9 +675,10 @@ static int tile_launch(const Product &p, uint32_t total, const Scales &sc, const
 }
 template <class S, class Epi>
 static int run_product(const Operand &a, const Operand &b, uint32_t m, uint32_t n, uint32_t k, uint32_t tile_n, const Scales &sc,
-                       const typename Epi::Args &epi, int sms, uint32_t *err, cudaStream_t st) {
+                       const typename Epi::Args &epi, int sms, uint32_t *err, cudaStream_t st, bool early = false) {
     Product p = {};
     AP_TRY((make_product<S, S::AMN, Epi>(&p, a, b, m, n, k, 1, tile_n, epi)));
+    p.grid.early = early;
     return tile_launch<S, Epi, tile::NoSecond>(p, p.grid.total, sc, epi, tile::Second<tile::NoSecond>{}, sms, err, st);
 }
 
@@ -820,7 +823,7 @@ static int backward_run(const LossCall &c, const BackwardPlan &p, uint8_t *ws, c
     float *part = reinterpret_cast<float *>(ws + p.p_off);
     PrepArgs pa{c.x, xc, c.ldx, p.ldx, c.target, grad, factor, c.rows, c.docs, c.dim, c.scale};
     AP_TRY(launch(grad_prep_kernel<T>, 1 + std::min<uint32_t>(ceil_div(c.rows, 8), 4 * (uint32_t)c.sms), pa, c.st));
-    const Operand x{xc, c.rows, c.dim, p.ldx};
+    const Operand x{xc, c.rows, c.dim, p.ldx}, given{c.x, c.rows, c.dim, c.ldx};
     for (uint32_t v0 = 0; v0 < c.docs; v0 += p.piece) {
         const uint32_t n = std::min(p.piece, c.docs - v0);
         const Operand w{static_cast<const T *>(c.w) + (size_t)v0 * c.ldw, n, c.dim, c.ldw};
@@ -829,7 +832,8 @@ static int backward_run(const LossCall &c, const BackwardPlan &p, uint8_t *ws, c
         ga.out.out = g; ga.out.ld = p.ldg; ga.out.m = c.rows; ga.out.n = n; ga.out.alpha = 1.f; ga.out.tma = 1; ga.out.padded = 1;
         ga.target = c.target; ga.loss = loss; ga.lse = lse; ga.grad = grad; ga.factor = factor; ga.col0 = v0; ga.docs = c.docs; ga.c = c.scale * kLog2e;
         const uint32_t tn = pick_n(kTileN, 32, CG, c.rows, n, ceil_div(c.dim, 64), c.sms);
-        AP_TRY((run_product<SG, GradEpi<T>>(x, w, c.rows, n, c.dim, tn, Scales{}, ga, c.sms, c.err, c.st)));
+        // from the rows as they were given: the logits are under way while the rows are prepared, the epilogue waits
+        AP_TRY((run_product<SG, GradEpi<T>>(given, w, c.rows, n, c.dim, tn, Scales{}, ga, c.sms, c.err, c.st, true)));
         typename StoreEpi<T>::Args wa{};
         wa.out = static_cast<T *>(dw) + (size_t)v0 * lddw; wa.ld = lddw; wa.m = n; wa.n = c.dim; wa.alpha = 1.f; wa.alpha_dev = factor + 1;
         wa.tma = aligned(wa.out, lddw * 2, 16);

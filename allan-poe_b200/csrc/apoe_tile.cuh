@@ -76,6 +76,7 @@ struct Shape {
 struct Grid {
     uint32_t tiles_m, tiles_n, group_m, kblocks, kper, total;   // kper: K blocks of a split (the last one may have fewer)
     uint32_t tile_n;                                            // columns of a tile: a multiple of 32, at most the shape's N
+    uint32_t early;                                             // the operands are complete before the kernel's predecessor has ended
 };
 __device__ __forceinline__ void locate(const Grid &g, uint32_t id, uint32_t &mi, uint32_t &ni, uint32_t &si) {
     const uint32_t per = g.tiles_m * g.tiles_n;
@@ -87,9 +88,10 @@ __device__ __forceinline__ void locate(const Grid &g, uint32_t id, uint32_t &mi,
     mi = grp * g.group_m + (r - ni * rows);
 }
 
-// Programmatic launch: the next kernel of the stream may start (as far as SMs are free) / wait until the kernels before this
-// one have ended and their writes are visible.  Every kernel of the dense operators does both, the wait before any access to
-// global memory, so kernels end in order.
+// Programmatic launch: wait until the kernels before this one have ended and their writes are visible / let the next kernel of
+// the stream start, as far as SMs are free.  Every kernel of the dense operators waits first and then lets the next one
+// start: so all that came before a kernel's predecessor is complete when the kernel starts, and it may read that (the
+// operators' inputs, once a kernel of the same call has run) before its own wait.  It writes nothing before.
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -314,7 +316,6 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
     };
 
-    pdl_launch();
     if (tid == 0) {
         for (int s = 0; s < S::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
         for (int s = 0; s < S::SF_SLOTS; ++s) { mbar_init(&sfull_bar[s], CG); mbar_init(&sempty_bar[s], 1); }   // an arrival per CTA
@@ -336,7 +337,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     if (CG == 2) cluster_sync();
     fence_after();
     const uint32_t tmem = tmem_base_s;
-    pdl_wait();
+    if (!grid.early || warp < kEpiWarps) pdl_wait();
+    if (tid == 0) pdl_launch();
 
     if (warp == kEpiWarps) {
         // ---------------- TMA producer (every CTA loads its own rows; the pair's leader counts the bytes of both) -----------
