@@ -605,9 +605,11 @@ static int launch(void (*kernel)(Args), uint32_t grid, const Args &args, cudaStr
 // What a tile costs, in K blocks of a full 16-bit tile (0.39 us on a pair of SMs): its K blocks, whose cost falls more slowly
 // than their columns, and 1.5 for its ends; a short K leaves the epilogue (2 us for 256 columns) to wait for.  Measured on
 // pairs at K = 4096, us per K block: 16 bits 0.26 / 0.29 / 0.35 / 0.39 at 64 / 128 / 224 / 256 columns, 8 bits 0.34 / 0.36 / 0.40
-// at 64 / 128 / 224.
-static double tile_cost(uint32_t tile_n, uint32_t kblocks, bool scaled = false) {
-    const double block = scaled ? (tile_n + 900) / 1100.0 : std::max((tile_n + 192) / 448.0, 0.66);
+// at 64 / 128 / 224.  One CTA per tile (few rows) waits for its columns from memory: 8 bits 0.36 / 0.48 / 0.64 / 0.72 at 32 / 128 /
+// 192 / 224 columns, 16 bits 0.50 / 0.65 / 0.82 at 128 / 192 / 256.
+static double tile_cost(int cg, uint32_t tile_n, uint32_t kblocks, bool scaled = false) {
+    const double block = cg == 1 ? std::max((tile_n + 75) / 160.0, scaled ? 0.92 : 0.66)
+                                 : scaled ? (tile_n + 900) / 1100.0 : std::max((tile_n + 192) / 448.0, 0.66);
     return std::max(kblocks * block + 1.5, 5.0 * tile_n / 256.0 + 1.0);
 }
 // Columns of a tile: as many as the shape allows, unless narrower tiles fill the rounds of the persistent grid better
@@ -617,7 +619,7 @@ static uint32_t pick_n(uint32_t most, uint32_t least, int cg, uint32_t m, uint32
     uint32_t best = most;
     double best_cost = 1e300;
     for (uint32_t w = most; w >= least; w -= 32) {
-        const double cost = (double)(((uint64_t)tiles_m * ceil_div(n, w) + groups - 1) / groups) * tile_cost(w, kblocks, scaled);
+        const double cost = (double)(((uint64_t)tiles_m * ceil_div(n, w) + groups - 1) / groups) * tile_cost(cg, w, kblocks, scaled);
         if (cost < best_cost * 0.985) { best_cost = cost; best = w; }
     }
     return best;
@@ -736,7 +738,7 @@ static Deal deal(uint32_t groups, uint32_t tx, uint32_t tw, double cx, double cw
 static Deal deal_of(uint32_t rows, uint32_t docs, uint32_t dim, const Cut &c, int sms) {
     const uint32_t cg = rows <= 128 ? 1 : 2, groups = std::max(1u, (uint32_t)sms / cg), cols = ceil_div(dim, c.n), kx = ceil_div(docs, 64);
     const uint32_t tx = ceil_div(rows, 128 * cg) * cols * c.splits, tw = ceil_div(docs, 128 * cg) * cols;
-    return deal(std::min(groups, tx + tw), tx, tw, tile_cost(c.n, ceil_div(kx, c.splits)), tile_cost(c.n, ceil_div(rows, 64)));
+    return deal(std::min(groups, tx + tw), tx, tw, tile_cost((int)cg, c.n, ceil_div(kx, c.splits)), tile_cost((int)cg, c.n, ceil_div(rows, 64)));
 }
 static Cut pick_cut(uint32_t rows, uint32_t docs, uint32_t dim, uint32_t most_splits, int sms) {
     // the narrowest tiles that still cover dim in as few columns of tiles as the widest do
