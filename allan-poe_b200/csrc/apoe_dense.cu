@@ -329,8 +329,8 @@ struct LseEpi {
     __device__ __forceinline__ void end() { if (row < a.m) a.part[(size_t)row * a.parts + part] = make_float2(top, sum); }
 };
 
-// One piece of G, times a power of two that brings the largest |grad| to 2^14 (f16 keeps small probabilities normal); a
-// rounding to 16 bits per element, the operands of the two products that follow.
+// One piece of G, times a power of two that brings its largest value to 2^14 (f16 keeps small ones normal); a rounding
+// to 16 bits per element, the operands of the two products that follow.
 template <class T>
 struct GradEpi {
     struct Args {
@@ -462,30 +462,37 @@ struct PrepArgs {
     void *xc;
     size_t ldx, ldxc;
     const uint32_t *target;
-    const float *grad;
+    const float *grad, *loss;
     float *factor;               // [0] the power of two, [1] scale / that
     uint32_t rows, docs, dim;
     float scale;
 };
 // A copy of the query rows with those that have no target set to zero (0 times whatever a padding row holds would not be 0
-// inside a product); block 0 also finds the factor of G from the largest |grad| of the rows that count.
+// inside a product); block 0 also finds the factor of G from the largest of its values in the rows that count.
 template <class T>
 __global__ void __launch_bounds__(256) grad_prep_kernel(const PrepArgs a) {
     tile::pdl_wait();
     tile::pdl_launch();
     if (blockIdx.x == 0) {
-        __shared__ float s[8];
-        float m = 0.f;
-        for (uint32_t i = threadIdx.x; i < a.rows; i += 256) if (a.target[i] < a.docs) m = fmaxf(m, fabsf(a.grad[i]));
+        // No |G| of a row exceeds that of its target, |grad| (1 - p): where a whole batch is nearly certain, so is the factor
+        __shared__ float s[2][8];
+        float top = 0.f, g = 0.f;
+        for (uint32_t i = threadIdx.x; i < a.rows; i += 256)
+            if (a.target[i] < a.docs) {
+                const float x = fabsf(a.grad[i]);
+                g = fmaxf(g, x);
+                top = fmaxf(top, x * -expm1f(-a.loss[i]));
+            }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
-        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = m;
+        for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(kAll, top, o)); g = fmaxf(g, __shfl_xor_sync(kAll, g, o)); }
+        if ((threadIdx.x & 31) == 0) { s[0][threadIdx.x >> 5] = top; s[1][threadIdx.x >> 5] = g; }
         __syncthreads();
         if (threadIdx.x == 0) {
-            for (int i = 1; i < 8; ++i) m = fmaxf(m, s[i]);
-            int e = 0;
-            if (m > 0.f && m < INFINITY) frexpf(m, &e);            // m <= 2^e
-            const int k = min(max(14 - e, -126), 126);
+            for (int i = 1; i < 8; ++i) { top = fmaxf(top, s[0][i]); g = fmaxf(g, s[1][i]); }
+            int e = 0, eg = 0;                                     // top <= 2^e, g <= 2^eg
+            if (top > 0.f && top < INFINITY) frexpf(top, &e);
+            if (g > 0.f && g < INFINITY) frexpf(g, &eg);
+            const int k = max(min(min(14 - e, 126), 120 - eg), -126);   // grad times the factor stays finite
             a.factor[0] = ldexpf(1.f, k);
             a.factor[1] = ldexpf(a.scale, -k);
         }
@@ -823,7 +830,7 @@ static int backward_run(const LossCall &c, const BackwardPlan &p, uint8_t *ws, c
     float *factor = reinterpret_cast<float *>(ws);
     T *xc = reinterpret_cast<T *>(ws + p.x_off), *g = reinterpret_cast<T *>(ws + p.g_off);
     float *part = reinterpret_cast<float *>(ws + p.p_off);
-    PrepArgs pa{c.x, xc, c.ldx, p.ldx, c.target, grad, factor, c.rows, c.docs, c.dim, c.scale};
+    PrepArgs pa{c.x, xc, c.ldx, p.ldx, c.target, grad, loss, factor, c.rows, c.docs, c.dim, c.scale};
     AP_TRY(launch(grad_prep_kernel<T>, 1 + std::min<uint32_t>(ceil_div(c.rows, 8), 4 * (uint32_t)c.sms), pa, c.st));
     const Operand x{xc, c.rows, c.dim, p.ldx}, given{c.x, c.rows, c.dim, c.ldx};
     for (uint32_t v0 = 0; v0 < c.docs; v0 += p.piece) {

@@ -386,6 +386,33 @@ def test_gradients_scale_with_the_losses_gradient():
     assert bool(torch.isfinite(gq).all()) and bool((gq[t >= 0] != 0).any())
 
 
+def test_nearly_certain_batches_keep_their_gradients_digits():
+    """A batch whose every row is certain (losses near 1e-9): its small G are held as exactly as large ones, so the f16 gradients,
+    brought back to ordinary size by the losses' gradient, are off by roundings only."""
+    dim, docs = 128, 40
+    g = gen(23)
+    d = torch.randn(docs, dim, generator=g, device=DEV)
+    d = (d / d.norm(dim=1, keepdim=True)).half()
+    t = torch.arange(docs, device=DEV, dtype=torch.int32)
+    q, scale = d.clone(), 36.0
+    loss, lse = apoe.softmax_loss_forward(q, d, t, scale)
+    assert float(loss.max()) < 1e-5
+    l = float(np.float32(scale)) * (q.double() @ d.double().t())
+    p = torch.softmax(l, 1)
+    away = torch.logsumexp(l.scatter(1, t.long()[:, None], -torch.inf), 1) - l.gather(1, t.long()[:, None])[:, 0]
+    p = p.scatter(1, t.long()[:, None], -torch.sigmoid(away)[:, None])
+    grad = (1.0 / loss.double()).float()                  # every row's coefficient near 1
+    dq, dd = apoe.softmax_loss_backward(q, d, t, loss, lse, grad, scale)
+    p = p * grad.double()[:, None]
+    eps = 4 * logit_bound(q, d, scale) + 4e-6             # exponentials: both logits and lse; the coefficient's loss likewise
+    for got, want, mass in ((dq, scale * (p @ d.double()), scale * (p.abs() @ d.double().abs())),
+                            (dd, scale * (p.t() @ q.double()), scale * (p.abs().t() @ q.double().abs()))):
+        u = U[torch.float16]
+        # G itself is rounded relative to the largest one of the batch: 2^-24 of 2^14 at the least
+        low = scale * 2.0 ** -38 * float(p.abs().max()) * docs
+        assert bool(((got.double() - want).abs() <= mass * (u + eps) + u * want.abs() + low + 2.0 ** -25).all())
+
+
 def test_single_rows_of_any_length():
     g = gen(19)
     for dim in (1, 7, 100, 333):
