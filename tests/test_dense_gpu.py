@@ -507,6 +507,48 @@ def test_ragged_scores_over_many_tiles(m, n, dtype):
         assert torch.equal(apoe.scaled_scores(qa, sa, qb, sb, out_dtype=dtype), first)
 
 
+def test_offsets_beyond_32_bits():
+    """More than 2^32 values on a side: the rows at the end are as right as those at the start."""
+    g = gen(81)
+    rows, dim = 4_200_000, 1024                                        # 4.3e9 values of f16
+    x = torch.empty(rows, dim, dtype=torch.float16, device=DEV)
+    x[:1000] = torch.randn(1000, dim, generator=g, device=DEV).half()
+    x[1000:-1000] = 0.5
+    x[-1000:] = torch.randn(1000, dim, generator=g, device=DEV).half()
+    q, s = apoe.quantize_rows(x)
+    for part in (slice(0, 50), slice(rows - 50, rows)):
+        want_q, want_s = plain_quantize(x[part])
+        assert torch.equal(q[part].cpu().double(), want_q) and torch.equal(s[part].cpu().long(), want_s)
+    few_q, few_s = q[-40:].clone(), s[-40:].clone()
+    out = apoe.scaled_scores(few_q, few_s, q, s, out_dtype=torch.float16)
+    check_scores(out[:, -500:], few_q, few_s, q[-500:], s[-500:])
+    del out
+    # the loss over these documents: the targets at the end, the gradient of the last rows
+    t = torch.arange(rows - 3, rows, device=DEV, dtype=torch.int32)
+    few = x[-3:].clone()
+    x[1000:-1000] *= 0.125
+    loss, lse = apoe.softmax_loss_forward(few, x, t, 0.01)
+    l = 0.01 * torch.cat([few.double() @ x[a:a + 400000].double().t() for a in range(0, rows, 400000)], 1)
+    want_lse = torch.logsumexp(l, 1)
+    bound = 2 * float(l.abs().max()) * (dim + 4) * 2.0 ** -23
+    assert float((lse.double() - want_lse).abs().max()) <= bound + 2.0 ** -20 * float(want_lse.abs().max())
+    grad = torch.full((3,), 1000.0, device=DEV)
+    _, dd = apoe.softmax_loss_backward(few, x, t, loss, lse, grad, 0.01)
+    p = torch.exp(l[:, -3:] - want_lse[:, None])
+    p -= torch.eye(3, device=DEV, dtype=torch.float64)
+    want = 10.0 * (p.t() @ few.double())                                # 0.01 * 1000
+    assert float((dd[-3:].double() - want).abs().max()) <= (3 * 2.0 ** -11 + 2 * bound + 1e-5) * 10.0 * float((p.abs().t() @ few.double().abs()).max())
+    del q, s, x, dd, l
+    # results beyond 2^32 values, on and off 16-byte rows
+    a, sa = apoe.quantize_rows(torch.randn(66000, 64, generator=g, device=DEV))
+    for n, ld in ((66000, 66000), (66000, 66001)):
+        room = torch.empty(66000, ld, dtype=torch.bfloat16, device=DEV)
+        apoe.scaled_scores(a, sa, a[:n], sa[:n], out=room[:, :n])
+        check_scores(room[-100:, n - 300:n], a[-100:], sa[-100:], a[n - 300:n], sa[n - 300:n])
+        check_scores(room[:100, :300], a[:100], sa[:100], a[:300], sa[:300])
+        del room
+
+
 def test_same_call_same_bits_on_any_stream():
     q, d, t, scale = loss_case(700, 3000, 256, torch.bfloat16, 31)
     grad = torch.full((700,), 1 / 700, device=DEV)
