@@ -646,7 +646,9 @@ struct Product {
 template <class S, bool AMN, class Epi>
 static int make_product(Product *p, const Operand &a, const Operand &b, uint32_t m, uint32_t n, uint32_t k, uint32_t splits, uint32_t tile_n,
                         const typename Epi::Args &epi) {
-    AP_TRY(make_map_2d(&p->a, S::KIND, a.base, a.rows, a.cols, a.ld, AMN ? 64 : 128));
+    // few rows: the rest of the 128 is not loaded (as zeros); what the products make of it is in rows that are not stored
+    p->grid.a_rows = S::CG == 1 && !AMN ? std::min<uint32_t>(128, ceil_div(m, 8) * 8) : 128;
+    AP_TRY(make_map_2d(&p->a, S::KIND, a.base, a.rows, a.cols, a.ld, AMN ? 64 : p->grid.a_rows));
     AP_TRY(make_map_2d(&p->b, S::KIND, b.base, b.rows, b.cols, b.ld, S::BMN ? 64 : tile_n / S::CG));
     Grid &g = p->grid;
     g.tiles_m = ceil_div(m, S::M);

@@ -76,6 +76,7 @@ struct Shape {
 struct Grid {
     uint32_t tiles_m, tiles_n, group_m, kblocks, kper, total;   // kper: K blocks of a split (the last one may have fewer)
     uint32_t tile_n;                                            // columns of a tile: a multiple of 32, at most the shape's N
+    uint32_t a_rows;                                            // rows of A a load brings (K-major): 128, fewer where there are fewer
     uint32_t early;                                             // the operands are complete before the kernel's predecessor has ended
 };
 __device__ __forceinline__ void locate(const Grid &g, uint32_t id, uint32_t &mi, uint32_t &ni, uint32_t &si) {
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         bool ok = true, free = true;
         auto load = [&](const CUtensorMap &ma, const CUtensorMap &mb, const Grid &gr, uint32_t t, auto amn) {
             constexpr bool AMN = decltype(amn)::value;
-            const uint32_t br = gr.tile_n / CG, bytes = (S::A_BYTES + (S::BMN ? (br + 63) / 64 * 8192 : br * 128)) * CG;
+            const uint32_t br = gr.tile_n / CG, bytes = ((AMN ? S::A_BYTES : gr.a_rows * 128) + (S::BMN ? (br + 63) / 64 * 8192 : br * 128)) * CG;
             uint32_t mi, ni, si;
             locate(gr, t, mi, ni, si);
             const int m0 = (int)(mi * S::M + rank * 128), n0 = (int)(ni * gr.tile_n + rank * br);
