@@ -921,6 +921,27 @@ extern "C" int ap_dense_check_status(int device, void *stream) {
     return fail(AP_ERR_DEVICE, "a dense operator raised error word %u (a bounded wait ran out)", ew);
 }
 
+namespace apoe {
+__global__ void dense_wait_probe_kernel(uint32_t polls, uint32_t *err) {
+    __shared__ uint64_t bar;
+    mbar_init(&bar, 1);
+    mbar_fence_init();
+    tile::wait(&bar, 0u, err, 39u, polls);        // nothing arrives: the wait runs out, the kernel ends
+}
+}  // namespace apoe
+
+extern "C" int ap_debug_dense_wait_timeout(int device, uint32_t polls, void *stream) {
+    if (polls > 4096) return fail(AP_ERR_ARG, "at most 4096 polls");
+    DeviceScope scope;
+    AP_TRY(scope.enter(device));
+    int sms;
+    uint32_t *err;
+    AP_TRY(device_facts(device, &sms, &err));
+    dense_wait_probe_kernel<<<1, 1, 0, (cudaStream_t)stream>>>(polls, err);
+    AP_CUDA(cudaGetLastError());
+    return AP_OK;
+}
+
 extern "C" int ap_quantize_rows_device(int device, uint32_t rows, uint32_t dim, uint32_t type, const void *src, uint64_t ld, uint8_t *q, uint64_t ldq,
                                        uint8_t *scale, uint64_t ld_scale, void *stream) {
     const int size = elem_size(type);

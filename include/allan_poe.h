@@ -448,6 +448,9 @@ int ap_debug_join_dense(ap_index *ix, uint32_t nodes, const uint32_t *plist, con
  * normally and the context stays usable.  ap_index_check_status then returns AP_ERR_DEVICE once. */
 int ap_debug_wait_timeout(ap_index *ix, uint32_t polls);
 
+/* The same for the dense operators: the device's error word is raised and ap_dense_check_status returns AP_ERR_DEVICE once. */
+int ap_debug_dense_wait_timeout(int device, uint32_t polls, void *stream);
+
 /* Profiling hook: the bandwidth the memory system gives the search's access pattern when the data is only fetched --
  * whole records of pseudo-random documents brought into shared memory by bulk copies, with the search kernel's CTA
  * count and shared-memory budget, `batches` batches per CTA (0 = 2000).  The ceiling, in gathered bytes per second, of

@@ -147,6 +147,16 @@ def test_scores_use_each_rows_and_blocks_own_scale(m):
     check_scores(apoe.scaled_scores(qa, sa, qb, sb, alpha=-0.37), qa, sa, qb, sb, alpha=float(np.float32(-0.37)))
 
 
+@pytest.mark.parametrize("up,down", [(100, -95), (-60, -50), (-110, 115), (60, 55)])
+@pytest.mark.parametrize("m", [5, 300])
+def test_scores_of_far_apart_scales(m, up, down):
+    """Scales whose product is ordinary (or small, or large) although each is near an end of its range."""
+    g = gen(14)
+    qa, sa = apoe.quantize_rows(torch.randn(m, 200, generator=g, device=DEV) * 2.0 ** up)
+    qb, sb = apoe.quantize_rows(torch.randn(90, 200, generator=g, device=DEV) * 2.0 ** down)
+    check_scores(apoe.scaled_scores(qa, sa, qb, sb), qa, sa, qb, sb)
+
+
 def test_scores_wide_narrow_and_many_tiles():
     """More tiles than SMs in every form: wide tiles for few rows, pairs of SMs, groups of row tiles."""
     g = gen(10)
@@ -594,6 +604,18 @@ def test_calls_are_captured_and_replayed():
     for a, b, c in zip(got, held, want):
         assert torch.equal(a, c) and torch.equal(b, c)
     apoe.dense_check_status()
+
+
+def test_a_wait_that_runs_out_is_reported_once():
+    """The error path of the bounded waits, without a fault: a kernel whose wait nothing ends gives up and returns."""
+    stream = torch.cuda.current_stream().cuda_stream
+    apoe._check(apoe.lib().ap_debug_dense_wait_timeout(0, 64, apoe.C.c_void_p(stream)))
+    with pytest.raises(apoe.ApoeError) as e:
+        apoe.dense_check_status()
+    assert e.value.code == 6 and "error word" in str(e.value)
+    apoe.dense_check_status()
+    q, s = apoe.quantize_rows(torch.ones(3, 128, device=DEV))          # the context stays usable
+    check_scores(apoe.scaled_scores(q, s, q, s), q, s, q, s)
 
 
 def test_train_pack_and_score_together():

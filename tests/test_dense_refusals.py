@@ -91,6 +91,10 @@ def test_loss_refuses(L):
     assert L.ap_softmax_loss_workspace(0, 4, 4, 4, 0, size) == 0 and size.value > 0
 
 
+def test_wait_probe_refuses_long_waits(L):
+    refused(1, "4096", L.ap_debug_dense_wait_timeout(0, 4097, None))
+
+
 def test_python_layer_refuses_what_is_not_on_the_device():
     x = torch.zeros(4, 64)
     for call in (lambda: apoe.quantize_rows(x), lambda: apoe.quantize_rows(x.double()),
