@@ -12,7 +12,7 @@
 //
 // Measured on the device: quantize 200 000 x 1024 f32 151 us (6.8 TB/s, bound by memory); scores 8192 x 65 536 x 1024 to bf16
 // 480-495 us (2.2 PFLOP/s; 2.6 without the epilogue); loss 8192 x 100 003 x 1024 bf16 1.01 ms (1.66 PFLOP/s, the tensor pipe 95 %
-// active); loss and gradients 4096 x 50 021 x 1024 bf16 1.11 ms (1.51 PFLOP/s with the logits made twice; 87 to 93 %).  Beside
+// active); loss and gradients 4096 x 50 021 x 1024 bf16 1.11 ms (1.51 PFLOP/s with the logits made twice; 89 to 95 %).  Beside
 // these the join of a row takes 3 to 7 us, the prepared copy and the last rounding 3 to 7 us each.
 #include <algorithm>
 #include <atomic>
