@@ -197,7 +197,7 @@ struct StoreEpi {
     float alpha;
     uint32_t row0 = 0, split = 0;
     __device__ __forceinline__ StoreEpi(const Args &args, tile::Staging &staging, const CUtensorMap *out, int lane_) : a(args), st(staging), map(out), lane(lane_) {
-        alpha = a.alpha_dev ? a.alpha * __ldg(a.alpha_dev) : a.alpha;
+        alpha = a.alpha_dev ? a.alpha * *a.alpha_dev : a.alpha;
     }
     __device__ __forceinline__ void ahead(uint32_t) {}
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t s, uint32_t) { row0 = r0; split = s; }
@@ -292,7 +292,7 @@ struct LseEpi {
     uint32_t row = 0, part = 0, tgt = 0, next = kNoTarget;
     float top = 0.f, sum = 0.f;
     __device__ __forceinline__ LseEpi(const Args &args, tile::Staging &, const CUtensorMap *, int lane_) : a(args), lane(lane_) {}
-    __device__ __forceinline__ void ahead(uint32_t r0) { next = r0 + lane < a.m ? __ldg(a.target + r0 + lane) : kNoTarget; }
+    __device__ __forceinline__ void ahead(uint32_t r0) { next = r0 + lane < a.m ? a.target[r0 + lane] : kNoTarget; }
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t, uint32_t p) {
         row = r0 + lane; part = p;
         tgt = next - a.col0;              // a target of another piece is none of this one's columns, and kNoTarget none at all
@@ -351,12 +351,12 @@ struct GradEpi {
     uint32_t tgt = 0, next = kNoTarget;
     float lse2 = 0.f, g = 0.f, at_target = 0.f, grad = 0.f, lse = 0.f, loss = 0.f, factor;
     __device__ __forceinline__ GradEpi(const Args &args, tile::Staging &staging, const CUtensorMap *out, int lane) : a(args), store(args.out, staging, out, lane) {
-        factor = __ldg(a.factor);
+        factor = *a.factor;
     }
     __device__ __forceinline__ void ahead(uint32_t r0) {
         const uint32_t row = min(r0 + store.lane, a.out.m - 1);      // past the last row: nothing is stored
-        next = __ldg(a.target + row);
-        grad = __ldg(a.grad + row); lse = __ldg(a.lse + row); loss = __ldg(a.loss + row);
+        next = a.target[row];
+        grad = a.grad[row]; lse = a.lse[row]; loss = a.loss[row];
     }
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t n0, uint32_t s, uint32_t p) {
         store.begin(r0, n0, s, p);
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs a) {
         const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx, *w = static_cast<const T *>(a.w) + (size_t)t * a.ldw;
         uint32_t i = lane * 8;
         for (; i + 8 <= a.dim; i += 256) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(x + i)), v = __ldg(reinterpret_cast<const uint4 *>(w + i));
+            const uint4 u = *reinterpret_cast<const uint4 *>(x + i), v = *reinterpret_cast<const uint4 *>(w + i);
             const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
             float d0 = 0.f, d1 = 0.f;
 #pragma unroll
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(256) grad_prep_kernel(const PrepArgs a) {
         const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx;
         T *o = static_cast<T *>(a.xc) + (size_t)row * a.ldxc;
         for (uint32_t i = lane * 8; i < a.dim; i += 256) {
-            if (i + 8 <= a.dim) *reinterpret_cast<uint4 *>(o + i) = live ? __ldg(reinterpret_cast<const uint4 *>(x + i)) : make_uint4(0u, 0u, 0u, 0u);
+            if (i + 8 <= a.dim) *reinterpret_cast<uint4 *>(o + i) = live ? *reinterpret_cast<const uint4 *>(x + i) : make_uint4(0u, 0u, 0u, 0u);
             else for (uint32_t k = i; k < a.dim; ++k) o[k] = live ? x[k] : Half16<T>::cast(0.f);
         }
     }

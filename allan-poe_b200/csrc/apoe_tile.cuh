@@ -93,6 +93,9 @@ __device__ __forceinline__ void locate(const Grid &g, uint32_t id, uint32_t &mi,
 // the stream start, as far as SMs are free.  Every kernel of the dense operators waits first and then lets the next one
 // start: so all that came before a kernel's predecessor is complete when the kernel starts, and it may read that (the
 // operators' inputs, once a kernel of the same call has run) before its own wait.  It writes nothing before.
+// Loads are plain ones, never non-coherent (ld.global.nc, __restrict__ on what is read): those are promised memory that nothing
+// writes while the kernel runs, and the predecessor of a kernel that has started early may still be writing what the
+// kernel reads after its wait (the scale bytes of rows quantised just before, the factor of the gradients).
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -487,8 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                     const uintptr_t p = (uintptr_t)(of_a ? scales.a + (size_t)row * scales.lda : scales.b + (size_t)row * scales.ldb) + kb;
                     const uintptr_t last = ((uintptr_t)(of_a ? scales.a_end : scales.b_end) - 1) & ~uintptr_t(3), q = p & ~uintptr_t(3);
                     places |= ((uint32_t)p & 3u) << (2 * j);
-                    lo[j] = __ldg(reinterpret_cast<const uint32_t *>(q));
-                    hi[j] = scales.words ? 0u : __ldg(reinterpret_cast<const uint32_t *>(q < last ? q + 4 : last));
+                    lo[j] = *reinterpret_cast<const uint32_t *>(q);
+                    hi[j] = scales.words ? 0u : *reinterpret_cast<const uint32_t *>(q < last ? q + 4 : last);
                 }
             };
             settle();
