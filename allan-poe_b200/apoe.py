@@ -609,7 +609,7 @@ def softmax_loss_backward(queries, docs, target, loss, lse, grad_loss, scale: fl
 
 def dense_check_status(device: int = 0, stream=None) -> None:
     """Waits for the stream (the device's current one by default) and raises ApoeError(6) when a bounded wait of an earlier
-    dense operator ran out."""
+    dense operator of this device, on any stream, ran out: once, on the first check after it."""
     T = _T or _torch()
     _check(lib().ap_dense_check_status(device, T.stream(device) if stream is None else stream))
 

@@ -907,18 +907,26 @@ static int check_loss(const char *what, uint32_t rows, uint32_t docs, uint32_t d
 
 using namespace apoe;
 
+namespace apoe {
+// Takes the error word: read and cleared in one step, so an error that another stream raises at the same moment is either in
+// what is taken or still there for the next check.
+__global__ void dense_take_error_kernel(uint32_t *taken) { *taken = atomicExch(&dense_error_word, 0u); }
+}  // namespace apoe
+
 extern "C" int ap_dense_check_status(int device, void *stream) {
     DeviceScope scope;
     AP_TRY(scope.enter(device));
     cudaStream_t st = (cudaStream_t)stream;
-    uint32_t ew = 0;
-    AP_CUDA(cudaMemcpyFromSymbolAsync(&ew, dense_error_word, 4, 0, cudaMemcpyDeviceToHost, st));
+    uint32_t *taken = nullptr, ew = 0;
+    AP_CUDA(cudaMallocAsync(&taken, sizeof(uint32_t), st));      // of this check alone: several may run at once
+    dense_take_error_kernel<<<1, 1, 0, st>>>(taken);
+    cudaError_t asked = cudaGetLastError();
+    if (asked == cudaSuccess) asked = cudaMemcpyAsync(&ew, taken, sizeof(uint32_t), cudaMemcpyDeviceToHost, st);
+    const cudaError_t freed = cudaFreeAsync(taken, st);
+    AP_CUDA(asked);
+    AP_CUDA(freed);
     AP_CUDA(cudaStreamSynchronize(st));
-    if (!ew) return AP_OK;
-    const uint32_t zero = 0;
-    AP_CUDA(cudaMemcpyToSymbolAsync(dense_error_word, &zero, 4, 0, cudaMemcpyHostToDevice, st));
-    AP_CUDA(cudaStreamSynchronize(st));
-    return fail(AP_ERR_DEVICE, "a dense operator raised error word %u (a bounded wait ran out)", ew);
+    return ew ? fail(AP_ERR_DEVICE, "a dense operator raised error word %u (a bounded wait ran out)", ew) : AP_OK;
 }
 
 namespace apoe {

@@ -349,8 +349,10 @@ int ap_exact_release(ap_index *ix);
 #define AP_TYPE_F32 0u
 #define AP_TYPE_F16 1u
 #define AP_TYPE_BF16 2u
-/* Waits for `stream` and reports (and clears) the device's error word: AP_ERR_DEVICE when a bounded wait of an earlier dense
- * operator ran out (its outputs are then incomplete), else AP_OK. */
+/* Waits for `stream` and reports (and clears, in one step) the device's error word: AP_ERR_DEVICE when a bounded wait of an
+ * earlier dense operator ran out (its outputs are then incomplete), else AP_OK.  The word is the device's: a check reports for
+ * the operators of every stream that have ended by then, once, so a caller with several streams takes one stream's report
+ * for all of them.  Not inside a capture. */
 int ap_dense_check_status(int device, void *stream);
 
 /* Rows in 8 bits: for each block of 128 values (the last one of a row may be shorter) e is the smallest integer >= -126 with
