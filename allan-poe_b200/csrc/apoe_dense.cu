@@ -28,6 +28,7 @@ using tile::Scales;
 
 constexpr uint32_t kNoTarget = 0xFFFFFFFFu;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.402823466e38f;       // maximum of nothing: below every logit, and differences to it are not NaN
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 
 __device__ uint32_t dense_error_word;   // raised by a kernel whose bounded wait ran out; read by ap_dense_check_status
@@ -278,11 +279,14 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { Pair d; asm("fma.
 __device__ __forceinline__ Pair add2(Pair a, Pair b) { Pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
 __device__ __forceinline__ Pair mul2(Pair a, Pair b) { Pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
 
-// Running maximum and sum of 2^(l log2 e) of a row over the columns of a tile, the target's column left out: the target's
-// own logit is computed apart and more exactly, because the loss is a difference against it.
+// Running maximum and sum of a row over the columns of a tile, the target's column left out: the target's own logit is computed
+// apart and more exactly, because the loss is a difference against it.  The maximum m is one of the products s themselves
+// (of -s for a negative scale), the sum one of 2^((s - m) |c|), c = scale * log2 e: a difference of products near each other is
+// exact, while a maximum of l = c s would be rounded, by more than an exponential can bear where logits are beyond 2^31.
 struct LseEpi {
+    static __device__ __forceinline__ float weight(float c) { return fmaxf(fabsf(c), 1.4e-45f); }   // 0: minus infinity has to stay that
     struct Args {
-        float2 *part;            // [rows][parts]: maximum and sum, in base 2
+        float2 *part;            // [rows][parts]: maximum and sum
         const uint32_t *target;
         uint32_t parts, m, n, col0;   // col0: document of this piece's first column
         float c;                 // scale * log2 e
@@ -296,10 +300,9 @@ struct LseEpi {
     __device__ __forceinline__ void begin(uint32_t r0, uint32_t, uint32_t, uint32_t p) {
         row = r0 + lane; part = p;
         tgt = next - a.col0;              // a target of another piece is none of this one's columns, and kNoTarget none at all
-        top = -1.0e30f; sum = 0.f;
+        top = kLowest; sum = 0.f;
     }
     __device__ __forceinline__ void chunk(uint32_t (&r)[32], uint32_t col) {
-        // the maximum of l = c s is |c| times the maximum of s with c's sign: one product-and-sum per exponential remains
         if (a.c < 0.f)
 #pragma unroll
             for (int j = 0; j < 32; ++j) r[j] ^= 0x80000000u;
@@ -317,17 +320,16 @@ struct LseEpi {
 #pragma unroll
             for (int k = 0; k < 4; ++k) m4[k] = max3(m4[k], __uint_as_float(r[j + k]), __uint_as_float(r[j + 4 + k]));
         const float m1 = max3(m4[0], __uint_as_float(r[28]), __uint_as_float(r[29])), m2 = max3(m4[1], __uint_as_float(r[30]), __uint_as_float(r[31]));
-        const float c = fmaxf(fabsf(a.c), 1e-30f);           // a scale of 0: what is left out stays at minus infinity
-        const float m = fmaxf(top, c * fmaxf(max3(m1, m2, m4[2]), m4[3]));
+        const float c = weight(a.c), m = fmaxf(top, fmaxf(max3(m1, m2, m4[2]), m4[3]));
         const Pair cc = pair(c, c), mm = pair(-m, -m);
         Pair s[4] = {pair(0.f, 0.f), pair(0.f, 0.f), pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-            const float2 x = split(fma2(pair(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), cc, mm));
+            const float2 x = split(mul2(add2(pair(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), mm), cc));
             s[(j >> 1) & 3] = add2(s[(j >> 1) & 3], pair(exp2_fast(x.x), exp2_fast(x.y)));
         }
         const float2 f = split(add2(add2(s[0], s[1]), add2(s[2], s[3])));
-        sum = sum * exp2_fast(top - m) + (f.x + f.y);
+        sum = sum * exp2_fast((top - m) * c) + (f.x + f.y);
         top = m;
     }
     __device__ __forceinline__ void finish() {}
@@ -435,33 +437,33 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs a) {
     tile::pdl_wait();
     tile::pdl_launch();
     if (row >= a.rows) return;
-    float top = -1.0e30f, sum = 0.f;
+    float top = kLowest, sum = 0.f;
+    const float c = LseEpi::weight(a.c);
+    const auto join = [&](float t2, float s2) {
+        const float m = fmaxf(top, t2);
+        sum = sum * exp2f((top - m) * c) + s2 * exp2f((t2 - m) * c);
+        top = m;
+    };
     const float2 *p = a.part + (size_t)row * a.parts;
     for (uint32_t i = lane; i < a.parts; i += 32) {
         const float2 e = p[i];
-        const float m = fmaxf(top, e.x);
-        sum = sum * exp2f(top - m) + e.y * exp2f(e.x - m);
-        top = m;
+        join(e.x, e.y);
     }
     if (lane == 0 && !a.first) {
         const float2 e = a.carry[row];
-        const float m = fmaxf(top, e.x);
-        sum = sum * exp2f(top - m) + e.y * exp2f(e.x - m);
-        top = m;
+        join(e.x, e.y);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float t2 = __shfl_xor_sync(kAll, top, o), s2 = __shfl_xor_sync(kAll, sum, o);
-        const float m = fmaxf(top, t2);
-        sum = sum * exp2f(top - m) + s2 * exp2f(t2 - m);
-        top = m;
+        join(t2, s2);
     }
     if (!a.last) { if (lane == 0) a.carry[row] = make_float2(top, sum); return; }
     float loss = 0.f, lse = 0.f;
     if (t < a.docs) {
-        // the logits were taken times c, a rounding of scale * log2 e: the maximum is put right, the sum holds differences only
-        const double at = (double)a.scale * dot, exact = a.c != 0.f ? (double)a.scale * 1.4426950408889634 / (double)a.c : 1.0;
-        const float z = (float)(((double)top * exact + log2((double)sum)) * 0.6931471805599453 - at);   // one document: minus infinity, loss 0
+        // c is a rounding of scale * log2 e, but the sum holds differences only
+        const double at = (double)a.scale * dot;
+        const float z = (float)(fabs((double)a.scale) * (double)top + log2((double)sum) * 0.6931471805599453 - at);   // one document: minus infinity, loss 0
         loss = z > 0.f ? z + log1pf(expf(-z)) : log1pf(expf(z));  // a NaN stays one
         lse = (float)(at + (double)loss);
     } else if (t != kNoTarget) loss = lse = __int_as_float(0x7FFFFFFF);
