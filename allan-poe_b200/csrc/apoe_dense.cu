@@ -734,12 +734,15 @@ static size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
 struct ForwardPlan { uint32_t piece, parts; size_t part_bytes, bytes; };
 // narrow tiles only where few documents leave SMs without work: the partial results of a row grow with their number
 static uint32_t least_n(uint32_t docs) { return docs <= 16384 ? 32 : 128; }
-// The tiles' maxima and sums (8 bytes per row and half a tile) of at most 64 MB of documents at a time
+// The tiles' maxima and sums, 8 bytes per row and half a tile, by pieces of the documents: at most 64 MB, or 512 bytes a row where
+// that is more (from 131 072 rows on).  A piece has at least 8192 documents (with pieces of 1024, 2^20 x 4096 x 128 took 3.16 ms
+// instead of 2.46), and where that many in narrow tiles would need more, its tiles are wider: the row tiles alone fill the SMs.
 static ForwardPlan forward_plan(uint32_t rows, uint32_t docs) {
     ForwardPlan p;
-    const uint32_t least = least_n(docs);
-    const uint64_t fit = (64ull << 20) / ((uint64_t)rows * 16) * least;
-    p.piece = (uint32_t)std::min<uint64_t>((uint64_t)ceil_div(docs, kTileN) * kTileN, std::max<uint64_t>(fit, 32 * kTileN));
+    const uint64_t fit = (64ull << 20) / ((uint64_t)rows * 16);         // tiles of a row in 64 MB
+    uint32_t least = least_n(docs);
+    while (least < kTileN && fit * least < std::min<uint64_t>(docs, 32 * kTileN)) least *= 2;
+    p.piece = (uint32_t)std::min<uint64_t>((uint64_t)ceil_div(docs, kTileN) * kTileN, std::max<uint64_t>(fit * least, 32 * kTileN));
     p.parts = 2 * ceil_div(std::min(p.piece, docs), least);
     p.part_bytes = round256((size_t)rows * p.parts * 8);
     p.bytes = p.part_bytes + round256((size_t)rows * 8);
@@ -780,7 +783,8 @@ static Cut pick_cut(uint32_t rows, uint32_t docs, uint32_t dim, uint32_t most_sp
 struct BackwardPlan { uint32_t piece, splits; bool direct; size_t ldx, ldg, ldp, x_off, g_off, p_off, bytes; };
 static BackwardPlan backward_plan(uint32_t rows, uint32_t docs, uint32_t dim, int sms) {
     BackwardPlan p;
-    // documents per piece: G of about 512 MB, at least 2048 documents (4096 x 50 021 x 1024, both gradients:
+    // documents per piece: G of at most 512 MB, or 4096 bytes a row where that is more: at least 2048 documents, 4 GB at 2^20
+    // rows (4096 x 50 021 x 1024, both gradients:
     // 1.15 ms with 32 MB, 1.10 with 128 MB, 1.06 with 512 MB: every piece adds to the sums of dX once more)
     const uint64_t most = std::max<uint64_t>(8, (512ull << 20) / ((uint64_t)rows * 2) / kTileN);
     p.piece = (uint32_t)std::min<uint64_t>(most, ceil_div(docs, kTileN)) * kTileN;
@@ -815,7 +819,8 @@ static int forward_run(const LossCall &c, const ForwardPlan &p, uint8_t *ws, flo
     for (uint32_t v0 = 0; v0 < c.docs; v0 += p.piece) {
         const uint32_t n = std::min(p.piece, c.docs - v0);
         const Operand w{static_cast<const T *>(c.w) + (size_t)v0 * c.ldw, n, c.dim, c.ldw};
-        const uint32_t tn = pick_n(kTileN, least_n(c.docs), CG, c.rows, n, ceil_div(c.dim, 64), c.sms);
+        const uint32_t least = std::max(least_n(c.docs), ceil_div(ceil_div(n, p.parts / 2), 32) * 32);     // as many tiles as there is room for
+        const uint32_t tn = pick_n(kTileN, least, CG, c.rows, n, ceil_div(c.dim, 64), c.sms);
         LseEpi::Args ea{part, c.target, 2 * ceil_div(n, tn), c.rows, n, v0, c.scale * kLog2e};
         AP_TRY((run_product<S, LseEpi>(x, w, c.rows, n, c.dim, tn, Scales{}, ea, c.sms, c.err, c.st)));
         JoinArgs ja{part, carry, c.x, c.w, c.ldx, c.ldw, c.target, loss, lse, c.rows, c.docs, c.dim, ea.parts, v0 == 0 ? 1u : 0u,
