@@ -487,6 +487,8 @@ def _matrix(name, t, device, dtypes):
     if len(stride) != 2 or not t.is_cuda or (device >= 0 and t.get_device() != device) or t.dtype not in dtypes:
         _bad(name, t, device, dtypes)
     rows, cols = t.shape
+    if rows > 0xFFFFFFFF or cols > 0xFFFFFFFF:      # ctypes would cut them to their low 32 bits without a word
+        raise ApoeError(4, f"{name}: {rows} x {cols}: fewer than 2^32 rows and values a row are supported")
     ld, step = stride
     if step != 1 and cols > 1:
         _bad(name, t, device, dtypes)
