@@ -725,6 +725,9 @@ static int device_facts(int device, int *sms, uint32_t **err) {
     return AP_OK;
 }
 static bool aligned(const void *p, uint64_t stride_bytes, uint64_t to) { return (uintptr_t)p % to == 0 && stride_bytes % to == 0; }
+static bool words(const void *a, const void *b = nullptr, const void *c = nullptr, const void *d = nullptr) {   // all on 4-byte boundaries
+    return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) & 3) == 0;
+}
 static int elem_size(uint32_t type) { return type == AP_TYPE_F32 ? 4 : (type == AP_TYPE_F16 || type == AP_TYPE_BF16) ? 2 : 0; }
 
 // ---- loss: how the work is cut ------------------------------------------------------------------------------------------
@@ -1040,6 +1043,7 @@ extern "C" int ap_softmax_loss_forward_device(int device, uint32_t rows, uint32_
                                               void *workspace, size_t workspace_bytes, void *stream) {
     AP_TRY(check_loss("softmax loss", rows, docs, dim, type, queries, ldq, documents, ldd, target, scale));
     if (!loss || !lse || !workspace) return fail(AP_ERR_ARG, "softmax loss: null argument");
+    if (!words(target, loss, lse)) return fail(AP_ERR_ARG, "softmax loss: target, loss and lse start on 4-byte boundaries");
     const ForwardPlan p = forward_plan(rows, docs);
     if (workspace_bytes < p.bytes) return fail(AP_ERR_ARG, "softmax loss: the workspace has %zu bytes, %zu are needed", workspace_bytes, p.bytes);
     if ((uintptr_t)workspace % 256) return fail(AP_ERR_ARG, "softmax loss: the workspace starts on a 256-byte boundary");
@@ -1058,6 +1062,7 @@ extern "C" int ap_softmax_loss_backward_device(int device, uint32_t rows, uint32
                                                uint64_t ldgd, void *workspace, size_t workspace_bytes, void *stream) {
     AP_TRY(check_loss("softmax loss gradient", rows, docs, dim, type, queries, ldq, documents, ldd, target, scale));
     if (!loss || !lse || !grad_loss || !grad_queries || !grad_documents || !workspace) return fail(AP_ERR_ARG, "softmax loss gradient: null argument");
+    if (!words(target, loss, lse, grad_loss)) return fail(AP_ERR_ARG, "softmax loss gradient: target, loss, lse and grad_loss start on 4-byte boundaries");
     if (ldgq < dim || ldgd < dim) return fail(AP_ERR_ARG, "softmax loss gradient: a row stride is shorter than a row");
     if (!aligned(grad_queries, ldgq * 2, 8) || (uintptr_t)grad_documents % 2) return fail(AP_ERR_ARG, "softmax loss gradient: rows of the queries' gradient start on 8-byte boundaries");
     DeviceScope scope;

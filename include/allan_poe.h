@@ -386,8 +386,9 @@ int ap_scaled_scores_device(int device, uint32_t dim, const ap_scaled_rows *a, c
  *   grad_documents = scale * G^T * queries.
  * lse is a float: its rounding, 2^-24 of its size, is an error of the same size of every probability of the row (an f16
  * step where logits reach some thousands, 0.5 at 2^23; beyond that the gradients mean nothing, the loss does).
- * Rows of grad_queries start on 8-byte boundaries.  workspace: device memory on a 256-byte boundary, at least as many bytes as
- * ap_softmax_loss_workspace gives for the call (backward = 0 or 1); its contents mean nothing before or after.
+ * target, loss, lse and grad_loss start on 4-byte boundaries, rows of grad_queries on 8-byte ones.  workspace: device memory
+ * on a 256-byte boundary, at least as many bytes as ap_softmax_loss_workspace gives for the call (backward = 0 or 1); its
+ * contents mean nothing before or after.
  * At least one query, document and value; at most 2^20, 2^30 and 2^16. */
 int ap_softmax_loss_workspace(int device, uint32_t rows, uint32_t docs, uint32_t dim, int backward, size_t *bytes);
 int ap_softmax_loss_forward_device(int device, uint32_t rows, uint32_t docs, uint32_t dim, uint32_t type, const void *queries,
