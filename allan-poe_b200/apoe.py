@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import os
+import warnings
 
 import numpy as np
 
@@ -461,6 +462,7 @@ class _Torch:
         self.f32, self.f16, self.bf16, self.f8, self.u8 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn, torch.uint8
         self.i32, self.u32 = torch.int32, torch.uint32
         self.types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+        self.grad_enabled = torch.is_grad_enabled
         self.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
@@ -577,8 +579,13 @@ def _workspace_bytes(device, rows, n, dim, backward):
 
 def softmax_loss_forward(queries, docs, target, scale: float = 1.0):
     """Softmax loss of queries over all documents without holding the matrix of scores: (loss, lse), float32 [rows].
-    queries [rows, dim] and docs [n, dim]: float16 or bfloat16; target: int32 document ids, -1 = the row takes no part."""
+    queries [rows, dim] and docs [n, dim]: float16 or bfloat16; target: int32 document ids, -1 = the row takes no part.
+    Autograd records nothing: gradients come from `softmax_loss_backward` alone.  Vectors that require gradients give a
+    warning; detached ones, or a call under torch.no_grad(), give none."""
     T = _T or _torch()
+    if (queries.requires_grad or docs.requires_grad) and T.grad_enabled():
+        warnings.warn("softmax_loss_forward takes no part in autograd: the gradients of queries and docs come from softmax_loss_backward "
+                      "(detach them, or call under torch.no_grad())", stacklevel=2)
     args = _loss_args(T, queries, docs, target)
     device, rows, n, dim = args[:4]
     size = _workspace_bytes(device, rows, n, dim, 0)

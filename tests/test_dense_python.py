@@ -1,4 +1,6 @@
 """What the Python layer of the dense operators settles before any device work (no GPU needed)."""
+import warnings
+
 import pytest
 import torch
 
@@ -37,3 +39,23 @@ def test_counts_beyond_32_bits_are_refused(rows):
         with pytest.raises(apoe.ApoeError) as e:
             call()
         assert e.value.code == 4 and "2^32" in str(e.value)
+
+
+def test_a_loss_that_records_no_gradients_says_so():
+    """The loss takes no part in autograd: inputs that require gradients would lose them silently where it is one term of a sum."""
+    targets = torch.zeros(4, dtype=torch.int32)
+    plain, wants = torch.zeros(4, 64).half(), torch.zeros(4, 64).half().requires_grad_()
+
+    def call(queries, docs):
+        with pytest.raises(apoe.ApoeError):            # host tensors: the call itself is refused
+            apoe.softmax_loss_forward(queries, docs, targets)
+
+    for pair in ((wants, plain), (plain, wants), (wants, wants)):
+        with pytest.warns(UserWarning, match="softmax_loss_backward"):
+            call(*pair)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        call(plain, plain)
+        call(wants.detach(), wants.detach())
+        with torch.no_grad():
+            call(wants, wants)
