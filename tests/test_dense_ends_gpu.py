@@ -111,3 +111,87 @@ def test_loss_of_large_logits_of_both_signs(rows, size):
         assert float((loss.double() - want_loss).abs().max()) <= 2 * tol
         assert float((lse.double() - want_lse).abs().max()) <= 2 * tol
         assert float(want_loss.max()) > 100 * tol
+
+
+def whole(rows, cols, g, dtype, share):
+    """-1, 0 and 1, so few of them that sums stay small."""
+    x = torch.randint(-1, 2, (rows, cols), generator=g, device=DEV).to(dtype)
+    return x * (torch.rand(rows, cols, generator=g, device=DEV) < share).to(dtype)
+
+
+@pytest.mark.parametrize("m,n,dim", [(3, 70, 1536), (150, 333, 1537), (300, 500, 4096), (5, 40, 16400), (140, 90, 65536 + 128 * 5 + 7), (2, 9, 1 << 20), (130, 33, 1 << 20)])
+def test_scores_of_long_rows(m, n, dim):
+    """Many groups of scale bytes, each block with a scale of its own; the scores are whole numbers below 2^24, so equal."""
+    g = gen(dim + m)
+    ld = (dim + 15) // 16 * 16
+    blocks = -(-dim // 128)
+    qa = torch.zeros(m, ld, device=DEV).to(torch.float8_e4m3fn)[:, :dim]
+    qb = torch.zeros(n, ld, device=DEV).to(torch.float8_e4m3fn)[:, :dim]
+    a, b = (whole(r, dim, g, torch.float32, min(1.0, 30.0 / dim ** 0.5)) for r in (m, n))
+    qa.copy_(a), qb.copy_(b)
+    sa, sb = (torch.randint(127, 131, (r, blocks), generator=g, device=DEV).to(torch.uint8) for r in (m, n))
+    va, vb = (x.double() * torch.exp2(s.double() - 127.0).repeat_interleave(128, 1)[:, :dim] for x, s in ((a, sa), (b, sb)))
+    assert float((va.abs() @ vb.abs().t()).max()) < 2 ** 20
+    assert torch.equal(apoe.scaled_scores(qa, sa, qb, sb).double(), va @ vb.t())
+    apoe.dense_check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,docs,dim", [(32, 256, 1536), (130, 300, 1544), (200, 700, 4096), (20, 100, 8200), (129, 200, 65536), (4, 90, 65536)])
+def test_loss_and_gradients_of_long_rows(rows, docs, dim, dtype):
+    """Whole logits, so of the loss only the join's errors remain, and of the gradients the roundings of G and of the result."""
+    g = gen(dim + rows)
+    ld = (dim + 7) // 8 * 8
+    q, d = (torch.zeros(r, ld, dtype=dtype, device=DEV)[:, :dim] for r in (rows, docs))
+    share = min(1.0, 3.0 / dim ** 0.5)
+    q.copy_(whole(rows, dim, g, dtype, share)), d.copy_(whole(docs, dim, g, dtype, share))
+    t = torch.randint(0, docs, (rows,), generator=g, device=DEV).to(torch.int32)
+    t[rows // 2] = -1
+    scale, live = 0.5, t >= 0
+    l, want_loss, want_lse = plain_rows(q, d, t.clamp(min=0), scale)
+    assert float(l.abs().max()) < 64
+    loss, lse = apoe.softmax_loss_forward(q, d, t, scale)
+    assert float((loss.double() - want_loss)[live].abs().max()) <= 64 * 2.0 ** -22 + 1e-6      # roundings at the size of a logit
+    assert float((lse.double() - want_lse)[live].abs().max()) <= 64 * 2.0 ** -22 + 1e-6
+    grad = torch.rand(rows, generator=g, device=DEV) + 0.5
+    dq, dd = apoe.softmax_loss_backward(q, d, t, loss, lse, grad, scale)
+    apoe.dense_check_status()
+    p = torch.exp(l - want_lse[:, None])
+    p[torch.arange(rows, device=DEV), t.clamp(min=0).long()] = torch.expm1(-want_loss)
+    p *= torch.where(live, grad.double(), 0.0)[:, None]
+    u = U[dtype]
+    # each G: a rounding, and its exponential's error (lse and the exponent, 2^-17 at |logit| 64); sums of at most 700 terms
+    near = u + 2.0 ** -17 + 2.0 ** -19 + 700 * 2.0 ** -23
+    small = 2.0 ** -25 if dtype == torch.float16 else 0.0                                       # f16's smallest step, halved
+    for got, want, mass, other in ((dq, scale * (p @ d.double()), scale * (p.abs() @ d.double().abs()), d),
+                                   (dd, scale * (p.t() @ q.double()), scale * (p.abs().t() @ q.double().abs()), q)):
+        low = small + small * 2.0 ** -13 * 1.5 * scale * other.double().abs().sum(0, keepdim=True)   # G at 2^14: steps of 2^-24
+        assert bool(((got.double() - want).abs() <= mass * near * (1 + u) + u * want.abs() + low).all())
+    assert not dq[rows // 2].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gradients_of_certain_and_hopeless_rows(dtype):
+    """Losses from 1e-12 to 100 in one batch, every element of both gradients against its own bound: a rounding of each G, its
+    exponential's and the loss's relative error, the result's rounding; f16 holds G in steps of 2^-24 where the batch's largest
+    is near 2^14."""
+    dim, docs, scale = 64, 300, 50.0
+    g = gen(13)
+    d = torch.randn(docs, dim, generator=g, device=DEV)
+    d = d / d.norm(dim=1, keepdim=True)
+    t = torch.arange(64, device=DEV, dtype=torch.int32)
+    q, d = torch.cat([d[:32], -d[32:64]]).to(dtype), d.to(dtype)
+    loss, lse = apoe.softmax_loss_forward(q, d, t, scale)
+    l, want_loss, want_lse = plain_rows(q, d, t, scale)
+    assert float(want_loss.min()) < 1e-9 and float(want_loss.max()) > 50
+    dq, dd = apoe.softmax_loss_backward(q, d, t, loss, lse, torch.ones(64, device=DEV), scale)
+    p = torch.exp(l - want_lse[:, None])
+    p[torch.arange(64, device=DEV), t.long()] = torch.expm1(-want_loss)
+    most = float((q.double().abs() @ d.double().abs().t()).max()) * scale
+    eps = 4 * most * (dim + 4) * 2.0 ** -23 + 4e-6           # two logits and lse in every exponent, the loss's in the target's
+    u = U[dtype]
+    small = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for got, want, mass, other in ((dq, scale * (p @ d.double()), scale * (p.abs() @ d.double().abs()), d),
+                                   (dd, scale * (p.t() @ q.double()), scale * (p.abs().t() @ q.double().abs()), q)):
+        low = small + small * 2.0 ** -13 * scale * other.double().abs().sum(0, keepdim=True)
+        assert bool(((got.double() - want).abs() <= mass * (u + eps + 300 * 2.0 ** -23) * (1 + u) + u * want.abs() + low).all())

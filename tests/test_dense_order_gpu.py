@@ -1,5 +1,10 @@
 """Dense operators that follow each other without a pause: each kernel may start while the one before it is still writing what
-it reads (scale bytes, the gradients' factor, targets).  Buffers are used over and over with other contents."""
+it reads (scale bytes, the gradients' factor, targets).  Buffers are used over and over with other contents.  And the first
+calls of a process inside a capture."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -63,3 +68,37 @@ def test_gradients_of_one_call_take_their_own_factor(rows, docs, dim):
         for a, b in zip(got, want):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
     apoe.dense_check_status()
+
+
+FIRST = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch, apoe
+g = torch.Generator(device="cuda").manual_seed(1)
+q, d = (torch.randn(n, 128, generator=g, device="cuda").half() for n in (200, 500))
+t = torch.randint(0, 500, (200,), generator=g, device="cuda").to(torch.int32)
+grad = torch.full((200,), 0.5, device="cuda")
+def step():
+    loss, lse = apoe.softmax_loss_forward(q, d, t, 0.1)
+    dq, dd = apoe.softmax_loss_backward(q, d, t, loss, lse, grad, 0.1)
+    q8, sq = apoe.quantize_rows(q)
+    d8, sd = apoe.quantize_rows(d)
+    return loss, lse, dq, dd, sq, sd, apoe.scaled_scores(q8, sq, d8, sd)
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    held = step()
+for x in held: x.zero_()
+graph.replay()
+torch.cuda.synchronize()
+got = [x.clone() for x in held]
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+apoe.dense_check_status()
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    """Nothing has to have run before: a process whose first dense calls are made inside a capture."""
+    r = subprocess.run([sys.executable, "-c", FIRST, os.path.dirname(apoe.__file__)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
