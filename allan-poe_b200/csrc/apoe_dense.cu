@@ -11,9 +11,10 @@
 // one piece of the documents at a time.
 //
 // Measured on the device: quantize 200 000 x 1024 f32 151 us (6.8 TB/s, bound by memory); scores 8192 x 65 536 x 1024 to bf16
-// 480-495 us (2.2 PFLOP/s; 2.6 without the epilogue); loss 8192 x 100 003 x 1024 bf16 1.01 ms (1.66 PFLOP/s, the tensor pipe 95 %
-// active); loss and gradients 4096 x 50 021 x 1024 bf16 1.11 ms (1.51 PFLOP/s with the logits made twice; 89 to 95 %).  Beside
-// these the join of a row takes 3 to 7 us, the prepared copy and the last rounding 3 to 7 us each.
+// 473-491 us (2.2 PFLOP/s; 2.6 without the epilogue; 569 us per call back to back, under the power cap); loss 8192 x 100 003 x 1024
+// bf16 1.00-1.03 ms (1.65 PFLOP/s, the tensor pipe 95 % active); loss and gradients 4096 x 50 021 x 1024 bf16 1.10-1.13 ms
+// (1.5 PFLOP/s with the logits made twice; 89 to 95 %).  Beside these the join of a row takes 3 to 7 us, the prepared copy and
+// the last rounding 3 to 7 us each.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -735,7 +736,9 @@ constexpr uint32_t kTileN = 256;
 static size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
 
 struct ForwardPlan { uint32_t piece, parts; size_t part_bytes, bytes; };
-// narrow tiles only where few documents leave SMs without work: the partial results of a row grow with their number
+// Narrow tiles only where few documents leave SMs without work: the partial results of a row grow with their number.  Tiles down to
+// 32 columns instead of 128: 128 x 4096 x 1024 9.2 us instead of 10.2, 128 x 10 000 10.7 instead of 11.0; within 3 % of each
+// other from 256 rows on, the same from 20 000 documents on.
 static uint32_t least_n(uint32_t docs) { return docs <= 16384 ? 32 : 128; }
 // The tiles' maxima and sums, 8 bytes per row and half a tile, by pieces of the documents: at most 64 MB, or 512 bytes a row where
 // that is more (from 131 072 rows on).  A piece has at least 8192 documents (with pieces of 1024, 2^20 x 4096 x 128 took 3.16 ms
@@ -787,8 +790,8 @@ struct BackwardPlan { uint32_t piece, splits; bool direct; size_t ldx, ldg, ldp,
 static BackwardPlan backward_plan(uint32_t rows, uint32_t docs, uint32_t dim, int sms) {
     BackwardPlan p;
     // documents per piece: G of at most 512 MB, or 4096 bytes a row where that is more: at least 2048 documents, 4 GB at 2^20
-    // rows (4096 x 50 021 x 1024, both gradients:
-    // 1.15 ms with 32 MB, 1.10 with 128 MB, 1.06 with 512 MB: every piece adds to the sums of dX once more)
+    // rows.  Every piece adds to the sums of dX once more; both gradients with 32 / 128 / 512 MB: 4096 x 50 021 x 1024 0.95 / 0.87 /
+    // 0.81 ms, 4096 x 50 021 x 128 450 / 351 / 314 us, 2000 x 20 000 x 128 87 / 72 / 72 us.
     const uint64_t most = std::max<uint64_t>(8, (512ull << 20) / ((uint64_t)rows * 2) / kTileN);
     p.piece = (uint32_t)std::min<uint64_t>(most, ceil_div(docs, kTileN)) * kTileN;
     p.splits = pick_cut(rows, std::min(p.piece, docs), dim, 32, sms).splits;
